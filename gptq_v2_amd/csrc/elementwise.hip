@@ -151,10 +151,10 @@ __global__ __launch_bounds__(256) void rope_kernel(T *__restrict__ x, int64_t ro
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const float a0 = static_cast<float>(static_cast<T>(__fmul_rn(lo[i], cl[i])));
-            const float b0 = static_cast<float>(static_cast<T>(__fmul_rn(-hi[i], sl[i])));
+            const float b0 = static_cast<float>(static_cast<T>(__fmul_rn(hi[i], sl[i])));
             const float a1 = static_cast<float>(static_cast<T>(__fmul_rn(hi[i], chh[i])));
             const float b1 = static_cast<float>(static_cast<T>(__fmul_rn(lo[i], sh[i])));
-            olo[i] = static_cast<T>(__fadd_rn(a0, b0));
+            olo[i] = static_cast<T>(__fsub_rn(a0, b0));   // a - b is a + (-b), and rounding is symmetric
             ohi[i] = static_cast<T>(__fadd_rn(a1, b1));
         }
         store8(xp, olo);
