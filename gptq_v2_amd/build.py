@@ -11,7 +11,8 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "build")
 LIB = os.path.join(HERE, "lib", "libgptq_amd.so")
-SOURCES = ["gq_core.hip", "xtx.hip", "hessian.hip", "sgemm.hip", "quantize.hip", "pack.hip", "w4a16.hip", "wq_stream.hip", "gemm_nt.hip", "elementwise.hip"]
+SOURCES = ["gq_core.hip", "xtx.hip", "hessian.hip", "sgemm.hip", "quantize.hip", "pack.hip", "w4a16.hip", "wq_stream.hip", "gemm_nt.hip", "elementwise.hip",
+           "logprobs.hip", "kv_append.hip", "attention_paged.hip", "attention_prompt.hip"]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-fno-fast-math",
          # no packed fp32 instructions: some of their forms have given wrong results now and then on this chip
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",

@@ -1,0 +1,499 @@
+// Attention of a few query tokens per sequence over a paged cache of 8-bit keys and values (the layout and the scales
+// that kv_append.hip writes): a decoder's step for one new token, or for the several of a checked draft or a chunk.
+//
+// With K = ks[page] k8 and V = vs[page] v8, in powers of two (c = softmax scale * log2 e):
+//   y_t = c ks (q . k8_t) + log2 vs,  M = max y,  w_t = 2^(y_t - M),  O = sum_t w_t v8_t / sum_t w_t / vs
+// The value's scale sits in the exponent, so the weights that meet the codes on the matrix core are at most 1 whatever
+// the scales are, and the denominator takes it out again in 32 bits.
+//
+// A wave takes 64 tokens at a time, all from registers: S^T = K Q^T (16 x 16 x 32 tiles: tokens by query rows) and
+// O^T = V^T P^T.  Row 4 g + i of the S^T tile a stands for token 16 g + 4 a + i; lane group g then holds, as the tiles'
+// results, the weights of the 16 adjacent tokens 16 g .. 16 g + 15 of its query row -- exactly what it has to supply as
+// the operand P^T, and exactly the 16 bytes it loads of a row of V^T.  No value crosses lanes but for the maximum.
+// The rows are the query heads that share a kv head (times the tokens of the sequence); the cache is read once for
+// every 16 NQ of them.  e4m3 codes are exact in either 16-bit type: Q K^T runs in q's type, P V in fp16 (w <= 1 keeps
+// 11 bits there, against 8 in bf16).
+//
+// Bound by HBM: 2 head_dim bytes per cached token and kv head.  A long sequence is cut into runs of tokens for several
+// workgroups, whose (O, M, l) a second kernel joins.
+#include "gq_common.h"
+
+namespace {
+
+constexpr float PA_LOG2E = 1.44269504088896340736f;
+
+struct PagedArgs {
+    const void *q;
+    void *out;
+    int64_t q_tok, q_head, o_tok, o_head;   // strides in elements
+    const uint8_t *k_codes, *v_codes;
+    const float *k_scale, *v_scale;
+    const int32_t *table, *lens, *cu;       // cu NULL: one query token per sequence
+    float *part_o, *part_ml;                // partial results: [token][head][split][head_dim], [token][head][split][2]
+    int64_t n_tokens, n_pages, table_width;
+    int batch, n_heads, n_kv_heads, group, head_dim, page_log2, tiles_per_split, n_splits, n_items;
+    float scale;                            // softmax scale * log2 e
+};
+
+template <typename T> struct Mfma;
+template <> struct Mfma<_Float16> {
+    typedef f16x8 vec;
+    static __device__ __forceinline__ f32x4 run(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+    // 8 codes (two words) to the operand's type, exactly
+    static __device__ __forceinline__ f16x8 decode(unsigned lo, unsigned hi)
+    {
+        const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, false), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, true);
+        const f16x2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, false), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, true);
+        return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+    }
+};
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+template <> struct Mfma<__bf16> {
+    typedef bf16x8 vec;
+    static __device__ __forceinline__ f32x4 run(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ bf16x8 decode(unsigned lo, unsigned hi)
+    {
+        const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, true);
+        const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, true);
+        return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+    }
+};
+
+// Sequence, first row and token rows of a workgroup's item.  With cu, sequence b's row tiles start at item
+// cu[b] group / MR + b, which leaves each sequence room for all its tiles without the host knowing the lengths.
+struct Item {
+    int b, tile;
+    int64_t row0;   // first query token's row in q
+    int n;          // query tokens of the sequence; 0: nothing to do
+};
+
+__device__ __forceinline__ Item find_item(const PagedArgs &a, int item, int mr)
+{
+    if (!a.cu) {
+        const int tiles = (a.group + mr - 1) / mr;
+        const int b = item / tiles;
+        return {b, item - b * tiles, b, 1};
+    }
+    const auto start = [&](int s) { return (int64_t)a.cu[s] * a.group / mr + s; };
+    int lo = 0, hi = a.batch - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (start(mid) <= item) lo = mid;
+        else hi = mid - 1;
+    }
+    const int64_t row0 = a.cu[lo], n = (int64_t)a.cu[lo + 1] - row0, tile = item - start(lo);
+    if (row0 < 0 || n <= 0 || row0 + n > a.n_tokens || tile < 0 || tile * mr >= n * a.group) return {lo, 0, 0, 0};
+    return {lo, (int)tile, row0, (int)n};
+}
+
+template <int NC>
+struct Tile {
+    u32x4 k[4][NC], v[4 * NC];
+    float ks, vs;
+};
+
+template <typename T, int NC, int NQ>
+__global__ __launch_bounds__(256, NQ == 1 ? 2 : 1) void attention_paged_kernel(const PagedArgs a)
+{
+    typedef Mfma<T> MM;
+    typedef typename MM::vec vec;
+    constexpr int MR = 16 * NQ, DP = 64 * NC, DT = 4 * NC;
+    constexpr int LROW = DP + 4;   // padded row of the join buffer, in floats
+    __shared__ float sm_m[4][MR], sm_l[4][MR];
+    __shared__ __attribute__((aligned(16))) float sm_o[4][16 * LROW];
+
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, g = lane >> 4;
+    const int head_kv = blockIdx.x % a.n_kv_heads, split = blockIdx.y;
+    const Item it = find_item(a, blockIdx.x / a.n_kv_heads, MR);
+    if (it.n == 0) return;
+    const int d = a.head_dim, page = 1 << a.page_log2;
+    int64_t len = a.lens[it.b];
+    if (len < 0) len = 0;
+    const int64_t n_tiles = (len + 63) >> 6;
+    const int64_t t_lo = (int64_t)split * a.tiles_per_split;
+    const int64_t t_hi = n_tiles < t_lo + a.tiles_per_split ? n_tiles : t_lo + a.tiles_per_split;
+    if (split > 0 && t_lo >= n_tiles) return;
+
+    // this lane's query rows (column m of each 16-row tile) and the last position each may see
+    vec qf[NQ][2 * NC];
+    int64_t last[NQ];
+#pragma unroll
+    for (int nt = 0; nt < NQ; ++nt) {
+        const int r = it.tile * MR + 16 * nt + m, tok = r / a.group;
+        const bool live = tok < it.n;
+        last[nt] = live ? len - it.n + tok : -1;
+        const T *qp = (const T *)a.q + (it.row0 + (live ? tok : 0)) * a.q_tok + (int64_t)(head_kv * a.group + (r - tok * a.group)) * a.q_head;
+#pragma unroll
+        for (int s = 0; s < 2 * NC; ++s) {
+            const int ch = 64 * (s >> 1) + 16 * g + 8 * (s & 1);
+            u32x4 raw = {0, 0, 0, 0};
+            if (live && ch < d) raw = *reinterpret_cast<const u32x4 *>(qp + ch);
+            __builtin_memcpy(&qf[nt][s], &raw, 16);
+        }
+    }
+
+    bool bad = false;   // a token that should be there lies on no page
+    const int32_t *table = a.table + (int64_t)it.b * a.table_width;
+    const int64_t head_bytes = (int64_t)page * d;
+    const auto page_of = [&](int64_t tok) -> int64_t {   // -1: behind the sequence, or no page
+        if (tok >= len) return -1;
+        const int64_t i = tok >> a.page_log2;
+        const int64_t id = i < a.table_width ? (int64_t)table[i] : -1;
+        if (id < 0 || id >= a.n_pages) {
+            bad = true;
+            return -1;
+        }
+        return id;
+    };
+    const auto load = [&](int64_t t, Tile<NC> &w) {
+        const int64_t tk = t * 64 + 16 * (m >> 2), tv = t * 64 + 16 * g;
+        const int64_t pk = page_of(tk), pv = page_of(tv);
+        const int64_t bk = pk * a.n_kv_heads + head_kv, bv = pv * a.n_kv_heads + head_kv;
+        const uint8_t *kp = a.k_codes + bk * head_bytes + ((tk & (page - 1)) + (m & 3)) * d + 16 * g;
+        const uint8_t *vp = a.v_codes + bv * head_bytes + (int64_t)m * page + (tv & (page - 1));
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                w.k[i][c] = u32x4{0, 0, 0, 0};
+                if (pk >= 0 && 64 * c + 16 * g < d) w.k[i][c] = *reinterpret_cast<const u32x4 *>(kp + 4 * i * d + 64 * c);
+            }
+#pragma unroll
+        for (int t2 = 0; t2 < DT; ++t2) {
+            w.v[t2] = u32x4{0, 0, 0, 0};
+            if (pv >= 0 && 16 * t2 < d) w.v[t2] = *reinterpret_cast<const u32x4 *>(vp + 16 * t2 * page);
+        }
+        w.ks = pv >= 0 ? a.k_scale[bv] : 1.f;
+        w.vs = pv >= 0 ? a.v_scale[bv] : 1.f;
+    };
+
+    f32x4 o[NQ][DT];
+    float mx[NQ], l[NQ];
+#pragma unroll
+    for (int nt = 0; nt < NQ; ++nt) {
+        mx[nt] = -INFINITY;
+        l[nt] = 0.f;
+#pragma unroll
+        for (int t2 = 0; t2 < DT; ++t2) o[nt][t2] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    // tokens from here on are hidden from some row: behind the sequence, or after a query token of it
+    const int64_t partly = len - it.n + 1;
+
+    Tile<NC> cur, nxt;
+    int64_t t = t_lo + wave;
+    if (t < t_hi) load(t, cur);
+    for (; t < t_hi; t += 4) {
+        if (t + 4 < t_hi) load(t + 4, nxt);
+        f32x4 s[NQ][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+            for (int nt = 0; nt < NQ; ++nt) s[nt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const vec kf = MM::decode(cur.k[i][c][2 * h], cur.k[i][c][2 * h + 1]);
+#pragma unroll
+                    for (int nt = 0; nt < NQ; ++nt) s[nt][i] = MM::run(kf, qf[nt][2 * c + h], s[nt][i]);
+                }
+        }
+        const float vs = fmaxf(cur.vs, 1e-30f);   // a scale of 0 must not become an infinite weight
+        const float mul = a.scale * cur.ks, add = __builtin_amdgcn_logf(vs), inv = 1.f / vs;
+        const bool masked = (t + 1) * 64 > partly;
+        f16x8 p[NQ][2];
+#pragma unroll
+        for (int nt = 0; nt < NQ; ++nt) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float y = fmaf(s[nt][i][j], mul, add);
+                    if (masked && t * 64 + 16 * g + 4 * i + j > last[nt]) y = -INFINITY;
+                    s[nt][i][j] = y;
+                    top = fmaxf(top, y);
+                }
+            top = fmaxf(top, __shfl_xor(top, 16, 64));
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            if (__any(top > mx[nt])) {
+                const float to = fmaxf(top, mx[nt]);
+                const float f = mx[nt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx[nt] - to);
+                mx[nt] = to;
+                l[nt] *= f;
+#pragma unroll
+                for (int t2 = 0; t2 < DT; ++t2)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) o[nt][t2][j] *= f;
+            }
+            const float ref = mx[nt] == -INFINITY ? 0.f : mx[nt];
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float w = __builtin_amdgcn_exp2f(s[nt][i][j] - ref);
+                    sum += w;
+                    p[nt][i >> 1][4 * (i & 1) + j] = (_Float16)w;
+                }
+            l[nt] = fmaf(sum, inv, l[nt]);
+        }
+        bool apart = false;   // a NaN among the values of a tile that is not visible to every row
+        if (masked) {
+            const int64_t left = len - (t * 64 + 16 * g);   // of this lane's 16 tokens
+            bool nan = false;
+#pragma unroll
+            for (int t2 = 0; t2 < DT; ++t2)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const int64_t k = left - 4 * w;
+                    const unsigned keep = k >= 4 ? 0xffffffffu : (k <= 0 ? 0u : (1u << (8 * k)) - 1);
+                    const unsigned x = cur.v[t2][w] & keep;
+                    cur.v[t2][w] = x;
+                    // a byte is NaN where its low seven bits are all set: then adding 1 carries into the eighth
+                    nan |= (((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
+                }
+            apart = it.n > 1 && __any(nan);
+        }
+        if (!apart) {
+#pragma unroll
+            for (int t2 = 0; t2 < DT; ++t2)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const f16x8 vf = Mfma<_Float16>::decode(cur.v[t2][2 * u], cur.v[t2][2 * u + 1]);
+#pragma unroll
+                    for (int nt = 0; nt < NQ; ++nt) o[nt][t2] = Mfma<_Float16>::run(vf, p[nt][u], o[nt][t2]);
+                }
+        } else {
+            // 0 * NaN is NaN: one token at a time, added only to the rows that see it
+            for (int tok = 0; tok < 64; ++tok) {
+                if (t * 64 + tok >= len) break;
+#pragma unroll
+                for (int t2 = 0; t2 < DT; ++t2) {
+                    unsigned w[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        w[i] = (tok >> 4) == g && ((tok >> 2) & 3) == i ? cur.v[t2][i] & (0xffu << (8 * (tok & 3))) : 0u;
+#pragma unroll
+                    for (int nt = 0; nt < NQ; ++nt) {
+                        f32x4 x = Mfma<_Float16>::run(Mfma<_Float16>::decode(w[0], w[1]), p[nt][0], f32x4{0.f, 0.f, 0.f, 0.f});
+                        x = Mfma<_Float16>::run(Mfma<_Float16>::decode(w[2], w[3]), p[nt][1], x);
+                        if (t * 64 + tok <= last[nt]) o[nt][t2] += x;
+                    }
+                }
+            }
+        }
+        cur = nxt;
+    }
+
+    // join the four waves
+    const bool any_bad = __any(bad);
+#pragma unroll
+    for (int nt = 0; nt < NQ; ++nt) {
+        l[nt] += __shfl_xor(l[nt], 16, 64);
+        l[nt] += __shfl_xor(l[nt], 32, 64);
+        if (any_bad) l[nt] = NAN;
+        if (g == 0) {
+            sm_m[wave][16 * nt + m] = mx[nt];
+            sm_l[wave][16 * nt + m] = l[nt];
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int nt = 0; nt < NQ; ++nt) {
+        const int rm = 16 * nt + m;
+        const float all = fmaxf(fmaxf(sm_m[0][rm], sm_m[1][rm]), fmaxf(sm_m[2][rm], sm_m[3][rm]));
+        const float f = mx[nt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx[nt] - all);
+        if (nt > 0) __syncthreads();
+#pragma unroll
+        for (int t2 = 0; t2 < DT; ++t2) {
+            f32x4 x = o[nt][t2];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] *= f;
+            *reinterpret_cast<f32x4 *>(&sm_o[wave][m * LROW + 16 * t2 + 4 * g]) = x;
+        }
+        __syncthreads();
+        const int row = threadIdx.x >> 4, rr = 16 * nt + row, r = it.tile * MR + rr, tok = r / a.group;
+        if (tok >= it.n) continue;
+        const float ma = fmaxf(fmaxf(sm_m[0][rr], sm_m[1][rr]), fmaxf(sm_m[2][rr], sm_m[3][rr]));
+        float sum = 0.f;
+        for (int w = 0; w < 4; ++w) sum += sm_l[w][rr] * (sm_m[w][rr] == -INFINITY ? (sm_l[w][rr] == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(sm_m[w][rr] - ma));
+        const int head = head_kv * a.group + (r - tok * a.group);
+        const int64_t qrow = it.row0 + tok;
+        for (int ch = 4 * (threadIdx.x & 15); ch < d; ch += 64) {
+            f32x4 x = {0.f, 0.f, 0.f, 0.f};
+            for (int w = 0; w < 4; ++w) x += *reinterpret_cast<const f32x4 *>(&sm_o[w][row * LROW + ch]);
+            if (a.n_splits > 1) {
+                *reinterpret_cast<f32x4 *>(a.part_o + ((qrow * a.n_heads + head) * a.n_splits + split) * d + ch) = x;
+            } else {
+                // a row without a key is 0
+                T y[4];
+                for (int j = 0; j < 4; ++j) y[j] = (T)(sum == 0.f ? 0.f : x[j] / sum);
+                u32x2 raw;
+                __builtin_memcpy(&raw, y, 8);
+                *reinterpret_cast<u32x2 *>((T *)a.out + qrow * a.o_tok + (int64_t)head * a.o_head + ch) = raw;
+            }
+        }
+        if (a.n_splits > 1 && (threadIdx.x & 15) == 0) {
+            float *ml = a.part_ml + ((qrow * a.n_heads + head) * a.n_splits + split) * 2;
+            ml[0] = ma;
+            ml[1] = sum;
+        }
+    }
+}
+
+// Joins a row's partial results: O = sum_s 2^(M_s - M) O_s / sum_s 2^(M_s - M) l_s.  One wave per row.
+template <typename T>
+__global__ __launch_bounds__(256) void attention_paged_join_kernel(const PagedArgs a)
+{
+    const int lane = threadIdx.x & 63;
+    const int64_t idx = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (idx >= a.n_tokens * a.n_heads) return;
+    const int64_t tok = idx / a.n_heads;
+    const int head = (int)(idx - tok * a.n_heads);
+    int b = (int)tok;
+    if (a.cu) {
+        if (tok < a.cu[0] || tok >= a.cu[a.batch]) return;   // behind the last sequence: left as it is
+        int lo = 0, hi = a.batch - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (a.cu[mid] <= tok) lo = mid;
+            else hi = mid - 1;
+        }
+        b = lo;
+        if (a.cu[b + 1] <= tok || a.cu[b] < 0 || a.cu[b + 1] > a.n_tokens) return;   // not rising: the first kernel left it out
+    }
+    const int64_t len = a.lens[b] < 0 ? 0 : a.lens[b], n_tiles = (len + 63) >> 6;
+    const int64_t used64 = (n_tiles + a.tiles_per_split - 1) / a.tiles_per_split;
+    const int used = used64 < 1 ? 1 : (used64 > a.n_splits ? a.n_splits : (int)used64);
+    const float *ml = a.part_ml + idx * a.n_splits * 2;
+    const float *po = a.part_o + idx * a.n_splits * a.head_dim;
+    float top = -INFINITY;
+    for (int s = lane; s < used; s += 64) top = fmaxf(top, ml[2 * s]);
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+    const float ref = top == -INFINITY ? 0.f : top;
+    float sum = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+    const int ch = 4 * lane;
+    for (int s = 0; s < used; ++s) {
+        const float f = __builtin_amdgcn_exp2f(ml[2 * s] - ref);
+        sum += ml[2 * s + 1] * (ml[2 * s] == -INFINITY && ml[2 * s + 1] != 0.f ? 1.f : f);
+        if (ch < a.head_dim) {
+            const f32x4 v = *reinterpret_cast<const f32x4 *>(po + (int64_t)s * a.head_dim + ch);
+            for (int j = 0; j < 4; ++j) x[j] = fmaf(v[j], f, x[j]);
+        }
+    }
+    // fewer splits than the sequence has tokens for: the table is too narrow for its length
+    if (used64 > a.n_splits) sum = NAN;
+    if (ch < a.head_dim) {
+        T y[4];
+        for (int j = 0; j < 4; ++j) y[j] = (T)(sum == 0.f ? 0.f : x[j] / sum);
+        u32x2 raw;
+        __builtin_memcpy(&raw, y, 8);
+        *reinterpret_cast<u32x2 *>((T *)a.out + tok * a.o_tok + (int64_t)head * a.o_head + ch) = raw;
+    }
+}
+
+struct Plan {
+    int nq, n_splits, tiles_per_split;
+    int64_t n_items;
+};
+
+// Query rows per workgroup: as many 16-row tiles as a sequence has rows on average, up to 4.  Splits: enough
+// workgroups to fill the chip, runs of at least 256 tokens (one tile per wave), at most 64 of them.
+Plan paged_plan(int64_t n_tokens, int64_t batch, bool ragged, int n_heads, int n_kv_heads, int page, int64_t table_width)
+{
+    Plan p;
+    const int64_t group = n_heads / n_kv_heads;
+    const int64_t rows = ragged ? gq_cdiv(n_tokens * group, batch) : group;
+    p.nq = rows <= 16 ? 1 : (rows <= 32 ? 2 : 4);
+    const int mr = 16 * p.nq;
+    p.n_items = ragged ? n_tokens * group / mr + batch : batch * gq_cdiv(group, mr);
+    const int64_t tiles = gq_cdiv(table_width * page, 64), wgs = p.n_items * n_kv_heads;
+    int64_t splits = gq_cdiv(2048, wgs);
+    splits = std::min<int64_t>(splits, gq_cdiv(tiles, 4));
+    splits = std::max<int64_t>(1, std::min<int64_t>(splits, 64));
+    p.tiles_per_split = (int)std::max<int64_t>(4, gq_round_up(gq_cdiv(tiles, splits), 4));
+    p.n_splits = (int)std::max<int64_t>(1, gq_cdiv(tiles, p.tiles_per_split));
+    return p;
+}
+
+bool paged_sizes_ok(int64_t n_tokens, int64_t batch, int n_heads, int n_kv_heads, int head_dim, int page, int64_t table_width)
+{
+    return n_tokens >= 0 && n_tokens < ((int64_t)1 << 31) && batch >= 0 && batch < (1 << 24) && n_kv_heads > 0 && n_heads > 0 && n_heads <= 65536 &&
+           n_heads % n_kv_heads == 0 && head_dim >= 16 && head_dim <= 128 && head_dim % 16 == 0 &&
+           (page == 16 || page == 32 || page == 64 || page == 128) && table_width >= 0 && table_width < ((int64_t)1 << 24);
+}
+
+template <typename T>
+int launch_paged(const PagedArgs &a, const Plan &p, hipStream_t s)
+{
+    const dim3 grid((unsigned)(p.n_items * a.n_kv_heads), (unsigned)p.n_splits);
+#define GQ_PA(NC, NQ) hipLaunchKernelGGL((attention_paged_kernel<T, NC, NQ>), grid, dim3(256), 0, s, a)
+    if (a.head_dim <= 64) {
+        if (p.nq == 1) GQ_PA(1, 1);
+        else if (p.nq == 2) GQ_PA(1, 2);
+        else GQ_PA(1, 4);
+    } else {
+        if (p.nq == 1) GQ_PA(2, 1);
+        else if (p.nq == 2) GQ_PA(2, 2);
+        else GQ_PA(2, 4);
+    }
+#undef GQ_PA
+    GQ_LAUNCH_CHECK();
+    if (p.n_splits > 1) {
+        hipLaunchKernelGGL(attention_paged_join_kernel<T>, dim3((unsigned)gq_cdiv(a.n_tokens * a.n_heads, 4)), dim3(256), 0, s, a);
+        GQ_LAUNCH_CHECK();
+    }
+    return GQ_OK;
+}
+
+}  // namespace
+
+extern "C" size_t gq_attention_paged_workspace(int64_t n_tokens, int64_t batch, int ragged, int n_heads, int n_kv_heads, int head_dim, int page,
+                                               int64_t table_width)
+{
+    if (!paged_sizes_ok(n_tokens, batch, n_heads, n_kv_heads, head_dim, page, table_width) || n_tokens == 0 || batch == 0) return 0;
+    const Plan p = paged_plan(n_tokens, batch, ragged != 0, n_heads, n_kv_heads, page, table_width);
+    return p.n_splits == 1 ? 0 : (size_t)n_tokens * n_heads * p.n_splits * (head_dim + 4) * sizeof(float);
+}
+
+extern "C" int gq_attention_paged(void *out, int64_t out_token_stride, int64_t out_head_stride, const void *q, int64_t q_token_stride,
+                                  int64_t q_head_stride, int dtype, int64_t n_tokens, int n_heads, const void *k_codes, const void *v_codes,
+                                  const float *k_scale, const float *v_scale, int64_t n_pages, int n_kv_heads, int page, int head_dim,
+                                  const int32_t *block_table, int64_t table_width, const int32_t *seq_lens, const int32_t *cu_seqlens,
+                                  int64_t batch, float softmax_scale, void *workspace, size_t workspace_bytes, gq_stream_t stream)
+{
+    GQ_REQUIRE(dtype == GQ_F16 || dtype == GQ_BF16, "gq_attention_paged: dtype %d is neither fp16 (0) nor bf16 (1)", dtype);
+    GQ_REQUIRE(paged_sizes_ok(n_tokens, batch, n_heads, n_kv_heads, head_dim, page, table_width) && n_pages >= 0,
+               "gq_attention_paged: %d heads on %d, head_dim %d (a multiple of 16 up to 128), pages of %d (16, 32, 64 or 128): not supported", n_heads,
+               n_kv_heads, head_dim, page);
+    GQ_REQUIRE(cu_seqlens || n_tokens == batch, "gq_attention_paged: %lld tokens for %lld sequences need cu_seqlens", (long long)n_tokens,
+               (long long)batch);
+    GQ_REQUIRE(softmax_scale > 0.f && softmax_scale < INFINITY, "gq_attention_paged: the softmax scale must be positive and finite");
+    if (n_tokens == 0 || batch == 0) return GQ_OK;
+    GQ_REQUIRE(out && q && seq_lens && (table_width == 0 || block_table) && (n_pages == 0 || (k_codes && v_codes && k_scale && v_scale)),
+               "gq_attention_paged: NULL pointer");
+    GQ_REQUIRE(q_token_stride % 8 == 0 && q_head_stride % 8 == 0 && out_token_stride % 8 == 0 && out_head_stride % 8 == 0,
+               "gq_attention_paged: strides must be multiples of 8 elements");
+    GQ_REQUIRE((((uintptr_t)out | (uintptr_t)q | (uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)workspace) & 15) == 0,
+               "gq_attention_paged: pointers must be 16-byte aligned");
+    const Plan p = paged_plan(n_tokens, batch, cu_seqlens != nullptr, n_heads, n_kv_heads, page, table_width);
+    GQ_REQUIRE(p.n_items * n_kv_heads < ((int64_t)1 << 31), "gq_attention_paged: too many query rows for one call");
+    const size_t need = p.n_splits == 1 ? 0 : (size_t)n_tokens * n_heads * p.n_splits * (head_dim + 4) * sizeof(float);
+    if (workspace_bytes < need || (need && !workspace)) {
+        gq_set_error("gq_attention_paged: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+        return GQ_EWORKSPACE;
+    }
+    PagedArgs a;
+    a.q = q, a.out = out, a.q_tok = q_token_stride, a.q_head = q_head_stride, a.o_tok = out_token_stride, a.o_head = out_head_stride;
+    a.k_codes = (const uint8_t *)k_codes, a.v_codes = (const uint8_t *)v_codes, a.k_scale = k_scale, a.v_scale = v_scale;
+    a.table = block_table, a.lens = seq_lens, a.cu = cu_seqlens;
+    a.part_o = (float *)workspace;
+    a.part_ml = (float *)workspace + (size_t)n_tokens * n_heads * p.n_splits * head_dim;
+    a.n_tokens = n_tokens, a.n_pages = n_pages, a.table_width = table_width;
+    a.batch = (int)batch, a.n_heads = n_heads, a.n_kv_heads = n_kv_heads, a.group = n_heads / n_kv_heads, a.head_dim = head_dim;
+    a.page_log2 = __builtin_ctz((unsigned)page), a.tiles_per_split = p.tiles_per_split, a.n_splits = p.n_splits, a.n_items = (int)p.n_items;
+    a.scale = softmax_scale * PA_LOG2E;
+    return dtype == GQ_F16 ? launch_paged<_Float16>(a, p, (hipStream_t)stream) : launch_paged<__bf16>(a, p, (hipStream_t)stream);
+}

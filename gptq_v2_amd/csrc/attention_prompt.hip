@@ -1,0 +1,332 @@
+// Attention over whole prompts: packed sequences of different lengths, grouped heads, causal or not.
+//
+//   S = scale Q K^T (masked),  m = row max,  P = e^(S - m),  O = P V / sum P
+// in one pass over the keys: a running (m, l, O) per query row, O and l rescaled when m grows.
+//
+// A workgroup of 4 waves takes 128 query rows of one head, a wave 32 of them, 64 keys at a time.  Everything is
+// computed transposed, S^T = K Q^T and O^T = V^T P^T with 32 x 32 x 16 matrix instructions: a lane then holds, of its
+// query row (its column), tokens 8 i + 4 h + 0..3 of the keys (h = lane / 32), and that is what it supplies as the
+// operand P^T when the inner index is taken in that order -- the weights go from the first product to the second
+// without leaving their lane, the row's maximum needs one exchange between two lanes.  K and V tiles are copied to LDS
+// by the asynchronous copy, 16-byte chunks permuted within a row (by the row) so that both the row-wise reads of K and
+// the transposing reads of V (4 tokens x 16 channels per 16 lanes) touch all banks evenly.
+// Rows behind a sequence's end and channels behind head_dim are out of the buffer descriptor's range and arrive as 0.
+//
+// Bound by the matrix core: 4 head_dim flops per visible (query, key) pair, next to one exponential.
+#include <type_traits>
+
+#include "gq_common.h"
+
+namespace {
+
+constexpr float AP_LOG2E = 1.44269504088896340736f;
+constexpr int AP_Q = 128, AP_K = 64;
+constexpr unsigned AP_OUT_OF_RANGE = 0x80000000u;
+
+struct PromptArgs {
+    const void *q, *k, *v;
+    void *out;
+    int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head, o_tok, o_head;   // strides in elements
+    const int32_t *cu;   // NULL: one sequence
+    int64_t n_tokens;
+    int batch, n_heads, group, head_dim, n_items, causal;
+    float scale;         // softmax scale * log2 e
+};
+
+typedef __amdgpu_buffer_rsrc_t ap_rsrc_t;
+
+template <typename T> struct Mma;
+template <> struct Mma<_Float16> {
+    typedef f16x8 vec;
+    static constexpr unsigned EXPONENT_ONE = 0x04000400u;
+    static __device__ __forceinline__ f32x16 run(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+template <> struct Mma<__bf16> {
+    typedef bf16x8 vec;
+    static constexpr unsigned EXPONENT_ONE = 0x00800080u;
+    static __device__ __forceinline__ f32x16 run(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+
+// swizzle of a row's 16-byte chunks: the 8 rows that are read together spread over the 8 chunks of 128 bytes (rows of
+// 192 bytes alternate between the halves of 128 by themselves, so theirs is over 4)
+template <int DP>
+__device__ __forceinline__ int ap_swizzle(int row) { return DP == 96 ? (row >> 1) & 3 : row & 7; }
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256, 2) void attention_prompt_kernel(const PromptArgs a)
+{
+    typedef typename Mma<T>::vec vec;
+    constexpr int NCH = DP / 8;                       // 16-byte chunks of a row
+    constexpr int PIECES = AP_K * NCH / 256;          // copy instructions per wave and tile
+    constexpr int STEPS = DP / 16, DT = DP / 32;
+    __shared__ __attribute__((aligned(1024))) T sm_k[2][AP_K * DP], sm_v[2][AP_K * DP];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, h = lane >> 5;
+    // workgroups of one head group run on one XCD (consecutive blocks go round the 8) and share its L2; long tiles first
+    int head, item;
+    if ((a.n_heads & 7) == 0) {
+        const int per = a.n_heads >> 3, x = blockIdx.x & 7, i = blockIdx.x >> 3;
+        head = x * per + i % per;
+        item = i / per;
+    } else {
+        head = blockIdx.x % a.n_heads;
+        item = blockIdx.x / a.n_heads;
+    }
+    item = a.n_items - 1 - item;
+    int64_t row0 = 0, n = a.n_tokens;
+    int tile = item;
+    if (a.cu) {
+        // sequence b's tiles start at item cu[b] / 128 + b: room for all of them without the host knowing the lengths
+        const auto start = [&](int s) { return (int64_t)a.cu[s] / AP_Q + s; };
+        int lo = 0, hi = a.batch - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (start(mid) <= item) lo = mid;
+            else hi = mid - 1;
+        }
+        row0 = a.cu[lo];
+        n = (int64_t)a.cu[lo + 1] - row0;
+        const int64_t t = item - start(lo);
+        if (row0 < 0 || n <= 0 || row0 + n > a.n_tokens || t < 0 || t * AP_Q >= n) return;
+        tile = (int)t;
+    }
+    const int len = (int)n, q0 = tile * AP_Q;
+    const int d = a.head_dim, head_kv = head / a.group;
+    const int row = q0 + wave * 32 + col;            // this lane's query row in its sequence
+
+    vec qf[STEPS];
+    {
+        const T *qp = (const T *)a.q + (row0 + (row < len ? row : 0)) * a.q_tok + head * a.q_head;
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            u32x4 raw = {0, 0, 0, 0};
+            if (row < len && 16 * s + 8 * h < d) raw = *reinterpret_cast<const u32x4 *>(qp + 16 * s + 8 * h);
+            __builtin_memcpy(&qf[s], &raw, 16);
+        }
+    }
+
+    // what each lane copies of a tile: chunk `tid + 256 j` of the tile in LDS, from its row and unswizzled channel
+    const unsigned k_row = (unsigned)(a.k_tok * sizeof(T)), v_row = (unsigned)(a.v_tok * sizeof(T));
+    unsigned k_off[PIECES], v_off[PIECES];
+#pragma unroll
+    for (int j = 0; j < PIECES; ++j) {
+        const int i = tid + 256 * j, r = i / NCH, c = (i - r * NCH) ^ ap_swizzle<DP>(r);
+        k_off[j] = 8 * c < d ? r * k_row + 16 * c : AP_OUT_OF_RANGE;
+        v_off[j] = 8 * c < d ? r * v_row + 16 * c : AP_OUT_OF_RANGE;
+    }
+    const T *kb = (const T *)a.k + row0 * a.k_tok + head_kv * a.k_head, *vb = (const T *)a.v + row0 * a.v_tok + head_kv * a.v_head;
+    const auto stage = [&](int j, int buf) {
+        const int rows = len - j * AP_K < AP_K ? len - j * AP_K : AP_K;
+        const ap_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((void *)(kb + (int64_t)j * AP_K * a.k_tok), 0, (int)((rows - 1) * k_row + 2 * d), 0x00020000);
+        const ap_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((void *)(vb + (int64_t)j * AP_K * a.v_tok), 0, (int)((rows - 1) * v_row + 2 * d), 0x00020000);
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, GQ_LDS_PTR(void, &sm_k[buf][(wave * 64 + 256 * p) * 8]), 16, (int)k_off[p], 0, 0, 0);
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, GQ_LDS_PTR(void, &sm_v[buf][(wave * 64 + 256 * p) * 8]), 16, (int)v_off[p], 0, 0, 0);
+    };
+
+    f32x16 o[DT];
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[t][r] = 0.f;
+    float mx = -INFINITY, l = 0.f;
+    const int q_last = q0 + AP_Q - 1 < len - 1 ? q0 + AP_Q - 1 : len - 1;
+    const int n_tiles = ((a.causal ? q_last : len - 1) + AP_K) / AP_K;
+    // tiles that some row of this wave sees
+    const int my_last = q0 + wave * 32 + 31 < len - 1 ? q0 + wave * 32 + 31 : len - 1;
+    const int my_tiles = a.causal ? (my_last + AP_K) / AP_K : n_tiles;
+    // tiles before this one are visible to every row of the wave
+    const int first_masked = a.causal ? (q0 + wave * 32 + 1) / AP_K : len / AP_K;
+    const int see = a.causal ? (row < len - 1 ? row : len - 1) : len - 1;   // the last key this row sees
+
+    const auto compute = [&](auto masked, int j, const T *tk, const T *tv) {
+        f32x16 s[2];
+#pragma unroll
+        for (int tb = 0; tb < 2; ++tb) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[tb][r] = 0.f;
+            const int kr = 32 * tb + col, sw = ap_swizzle<DP>(kr);
+#pragma unroll
+            for (int st = 0; st < STEPS; ++st) {
+                const vec kf = *reinterpret_cast<const vec *>(tk + kr * DP + ((2 * st + h) ^ sw) * 8);
+                s[tb] = Mma<T>::run(kf, qf[st], s[tb]);
+            }
+        }
+        if (masked && j >= first_masked) {
+#pragma unroll
+            for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (j * AP_K + 32 * tb + 8 * (r >> 2) + 4 * h + (r & 3) > see) s[tb][r] = -INFINITY;
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) top = fmaxf(top, s[tb][r]);
+        top = fmaxf(top, __shfl_xor(top, 32, 64)) * a.scale;
+        if (__any(top > mx)) {
+            const float to = fmaxf(top, mx);
+            const float f = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - to);
+            mx = to;
+            l *= f;
+#pragma unroll
+            for (int t = 0; t < DT; ++t)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[t][r] *= f;
+        }
+        const float ref = mx == -INFINITY ? 0.f : mx;
+        vec p[4];
+#pragma unroll
+        for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float w = __builtin_amdgcn_exp2f(fmaf(s[tb][r], a.scale, -ref));
+                l += w;
+                p[2 * tb + (r >> 3)][r & 7] = static_cast<T>(w);
+            }
+        // V^T of channels 32 t .. and tokens 16 s2 + 4 h + 0..3, 16 s2 + 8 + 4 h + 0..3, as the weights have them
+        const auto read_v = [&](int t, int s2) {
+            vec vf;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int vr = 16 * s2 + 8 * half + 4 * h + ((lane >> 2) & 3), c0 = 32 * t + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+                const T *p0 = tv + vr * DP + (((c0 >> 3) ^ ap_swizzle<DP>(vr)) << 3) + (c0 & 7);
+                const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(GQ_LDS_PTR(s16x4, p0));
+                __builtin_memcpy((char *)&vf + 8 * half, &x, 8);
+            }
+            return vf;
+        };
+        bool apart = false;
+        if (masked && a.causal && j >= first_masked) {
+            // 0 * inf and 0 * NaN are NaN: an infinity or NaN among these values must not reach the rows before it.
+            // Adding one to an exponent field of all ones carries into the sign's place.
+            unsigned found = 0;
+#pragma unroll 1
+            for (int i = lane; i < AP_K * NCH; i += 64) {
+                const u32x4 x = *reinterpret_cast<const u32x4 *>(tv + i * 8);
+#pragma unroll
+                for (int w = 0; w < 4; ++w) found |= (x[w] & 0x7fff7fffu) + Mma<T>::EXPONENT_ONE;
+            }
+            apart = __any((found & 0x80008000u) != 0);
+        }
+        if (!masked || !apart) {
+#pragma unroll
+            for (int t = 0; t < DT; ++t)
+#pragma unroll
+                for (int s2 = 0; s2 < 4; ++s2) o[t] = Mma<T>::run(read_v(t, s2), p[s2], o[t]);
+            return;
+        }
+        // one token at a time, added only to the rows that see it
+#pragma unroll
+        for (int s2 = 0; s2 < 4; ++s2)
+#pragma unroll 1
+            for (int tok = 0; tok < 16; ++tok) {
+#pragma unroll
+                for (int t = 0; t < DT; ++t) {
+                    asm volatile("" ::: "memory");   // keep the reads here: held for all tokens they would cost the common path its registers
+                    vec vf = read_v(t, s2);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (8 * (i >> 2) + 4 * h + (i & 3) != tok) vf[i] = static_cast<T>(0.f);
+                    f32x16 x;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) x[r] = 0.f;
+                    x = Mma<T>::run(vf, p[s2], x);
+                    if (j * AP_K + 16 * s2 + tok <= see) {
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) o[t][r] += x[r];
+                    }
+                }
+            }
+    };
+
+    stage(0, 0);
+    // pairs of tiles that are visible to the whole workgroup, then those that may be masked
+    const int n_clear = (a.causal ? (q0 + 1) / AP_K : len / AP_K) & ~1;
+    int j = 0;
+    for (; j < n_clear; j += 2) {
+        __syncthreads();
+        stage(j + 1, 1);
+        compute(std::false_type(), j, sm_k[0], sm_v[0]);
+        __syncthreads();
+        if (j + 2 < n_tiles) stage(j + 2, 0);
+        compute(std::false_type(), j + 1, sm_k[1], sm_v[1]);
+    }
+    for (; j < n_tiles; j += 2) {
+        __syncthreads();
+        if (j + 1 < n_tiles) stage(j + 1, 1);
+        if (j < my_tiles) compute(std::true_type(), j, sm_k[0], sm_v[0]);
+        if (j + 1 >= n_tiles) break;
+        __syncthreads();
+        if (j + 2 < n_tiles) stage(j + 2, 0);
+        if (j + 1 < my_tiles) compute(std::true_type(), j + 1, sm_k[1], sm_v[1]);
+    }
+
+    l += __shfl_xor(l, 32, 64);
+    if (row >= len) return;
+    const float inv = 1.f / l;
+    T *op = (T *)a.out + (row0 + row) * a.o_tok + head * a.o_head;
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+            const int ch = 32 * t + 8 * r4 + 4 * h;
+            if (ch >= d) continue;
+            T y[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] = static_cast<T>(o[t][4 * r4 + i] * inv);
+            u32x2 raw;
+            __builtin_memcpy(&raw, y, 8);
+            *reinterpret_cast<u32x2 *>(op + ch) = raw;
+        }
+}
+
+template <typename T>
+int launch_prompt(const PromptArgs &a, hipStream_t s)
+{
+    const dim3 grid((unsigned)a.n_items * (unsigned)a.n_heads);
+#define GQ_AP(DP) hipLaunchKernelGGL((attention_prompt_kernel<T, DP>), grid, dim3(256), 0, s, a)
+    if (a.head_dim <= 64) GQ_AP(64);
+    else if (a.head_dim <= 96) GQ_AP(96);
+    else GQ_AP(128);
+#undef GQ_AP
+    GQ_LAUNCH_CHECK();
+    return GQ_OK;
+}
+
+}  // namespace
+
+extern "C" int gq_attention_prompt(void *out, int64_t out_token_stride, int64_t out_head_stride, const void *q, int64_t q_token_stride,
+                                   int64_t q_head_stride, const void *k, int64_t k_token_stride, int64_t k_head_stride, const void *v,
+                                   int64_t v_token_stride, int64_t v_head_stride, int dtype, int64_t n_tokens, int n_heads, int n_kv_heads,
+                                   int head_dim, const int32_t *cu_seqlens, int64_t batch, int causal, float softmax_scale, gq_stream_t stream)
+{
+    GQ_REQUIRE(dtype == GQ_F16 || dtype == GQ_BF16, "gq_attention_prompt: dtype %d is neither fp16 (0) nor bf16 (1)", dtype);
+    GQ_REQUIRE(head_dim >= 8 && head_dim <= 128 && head_dim % 8 == 0, "gq_attention_prompt: head_dim %d is not a multiple of 8 up to 128", head_dim);
+    GQ_REQUIRE(n_heads > 0 && n_kv_heads > 0 && n_heads % n_kv_heads == 0 && n_heads <= 65536, "gq_attention_prompt: %d query heads on %d", n_heads, n_kv_heads);
+    GQ_REQUIRE(n_tokens >= 0 && n_tokens < ((int64_t)1 << 30) && batch >= 0 && batch < (1 << 24), "gq_attention_prompt: bad number of tokens or sequences");
+    GQ_REQUIRE(cu_seqlens || batch == 1 || n_tokens == 0, "gq_attention_prompt: %lld sequences need cu_seqlens", (long long)batch);
+    GQ_REQUIRE(softmax_scale > 0.f && softmax_scale < INFINITY, "gq_attention_prompt: the softmax scale must be positive and finite");
+    if (n_tokens == 0 || batch == 0) return GQ_OK;
+    GQ_REQUIRE(out && q && k && v, "gq_attention_prompt: NULL pointer");
+    GQ_REQUIRE(out_token_stride % 8 == 0 && out_head_stride % 8 == 0 && q_token_stride % 8 == 0 && q_head_stride % 8 == 0 && k_token_stride % 8 == 0 &&
+                   k_head_stride % 8 == 0 && v_token_stride % 8 == 0 && v_head_stride % 8 == 0,
+               "gq_attention_prompt: strides must be multiples of 8 elements");
+    // a tile of 64 rows is addressed by 32-bit offsets, and a row must lie behind the one before it
+    GQ_REQUIRE(n_tokens == 1 || (k_token_stride >= head_dim && v_token_stride >= head_dim && k_token_stride <= (1 << 23) && v_token_stride <= (1 << 23)),
+               "gq_attention_prompt: token strides of k and v must be in head_dim..2^23");
+    GQ_REQUIRE((((uintptr_t)out | (uintptr_t)q | (uintptr_t)k | (uintptr_t)v) & 15) == 0, "gq_attention_prompt: pointers must be 16-byte aligned");
+    const int64_t n_items = cu_seqlens ? n_tokens / AP_Q + batch : gq_cdiv(n_tokens, AP_Q);
+    GQ_REQUIRE(n_items * n_heads < ((int64_t)1 << 31), "gq_attention_prompt: too many tokens for one call");
+    PromptArgs a;
+    a.q = q, a.k = k, a.v = v, a.out = out;
+    a.q_tok = q_token_stride, a.q_head = q_head_stride, a.k_tok = k_token_stride, a.k_head = k_head_stride;
+    a.v_tok = v_token_stride, a.v_head = v_head_stride, a.o_tok = out_token_stride, a.o_head = out_head_stride;
+    a.cu = cu_seqlens, a.n_tokens = n_tokens, a.batch = (int)batch, a.n_heads = n_heads, a.group = n_heads / n_kv_heads;
+    a.head_dim = head_dim, a.n_items = (int)n_items, a.causal = causal != 0, a.scale = softmax_scale * AP_LOG2E;
+    return dtype == GQ_F16 ? launch_prompt<_Float16>(a, (hipStream_t)stream) : launch_prompt<__bf16>(a, (hipStream_t)stream);
+}

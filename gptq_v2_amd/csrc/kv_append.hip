@@ -1,0 +1,358 @@
+// Appending keys and values to a paged cache of 8-bit numbers, with the rotary embedding applied on the way.
+//
+// The cache holds e4m3 codes in pages of `page` tokens, one scale per (page, kv head) and tensor:
+//   k_codes[n_pages][n_kv_heads][page][head_dim],  v_codes[n_pages][n_kv_heads][head_dim][page],  value = code * scale.
+// Keys lie by token and values by channel because the attention over the cache reads both as operands of the matrix
+// instruction whose inner index must be contiguous: channels for Q K^T, tokens for P V.
+//
+// Scales are powers of two, 2^e with the smallest e for which the page's largest finite magnitude a fits, a 2^-e <= 448.
+// That costs an e4m3 number no precision (its error is relative), and it makes a page that fills up token by token
+// well defined: when a new token needs a larger scale, the codes already there are re-expressed by a power of two,
+// which only moves their exponent -- exact but for codes that become subnormal (below 2^-6 of a page whose largest code
+// lies in (224, 448]).  Every value is rounded once from 32 bits: the rotated key never passes through 16 bits.
+//
+// One workgroup owns a (sequence's page, kv head, keys or values): it needs the largest magnitude before the first
+// store, and nobody else may touch the page while codes are re-expressed.  A thread holds 4 tokens x 8 channels in
+// registers between the two, so the input is read once where the page has no more than one such item per thread.
+// Bound by HBM for prompts (16-bit input in, one byte out), by launch and two dependent loads for single tokens.
+#include "gq_common.h"
+
+namespace {
+
+constexpr float E4M3_MAX = 448.f;
+constexpr int MIN_EXP = -100, MAX_EXP = 120;   // exponents of scales; MIN_EXP is a page of zeros
+
+struct AppendArgs {
+    const void *q, *k, *v;            // [n_tokens][heads][head_dim] by strides; q may be NULL
+    void *q_out;
+    int64_t q_tok, q_head, qo_tok, qo_head, k_tok, k_head, v_tok, v_head;   // strides in elements
+    uint8_t *k_codes, *v_codes;
+    float *k_scale, *v_scale;
+    const float *cos_t, *sin_t;       // [max_pos][rot / 2]
+    const int32_t *table, *past, *cu;   // cu NULL: one token per sequence
+    int64_t n_tokens, max_pos, n_pages, table_width;
+    int batch, n_heads, n_kv_heads, head_dim, page, rot, interleaved, n_items;
+};
+
+template <typename T>
+__device__ __forceinline__ void load8f(const T *p, float (&f)[8])
+{
+    const u32x4 raw = *reinterpret_cast<const u32x4 *>(p);
+    T v[8];
+    __builtin_memcpy(v, &raw, 16);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = static_cast<float>(v[i]);
+}
+
+template <typename T>
+__device__ __forceinline__ void store8f(T *p, const float (&f)[8])
+{
+    T v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = static_cast<T>(f[i]);
+    u32x4 raw;
+    __builtin_memcpy(&raw, v, 16);
+    *reinterpret_cast<u32x4 *>(p) = raw;
+}
+
+// 8 channels of one head at channel c0 < rot after the rotation, each product and the sum rounded in 32 bits
+template <typename T>
+__device__ __forceinline__ void load8_rotated(const T *head, int c0, const float *cos_r, const float *sin_r, int rot, int interleaved,
+                                              float (&f)[8])
+{
+    load8f(head + c0, f);
+    if (c0 >= rot) return;
+    if (interleaved) {
+        const f32x4 c = *reinterpret_cast<const f32x4 *>(cos_r + c0 / 2), s = *reinterpret_cast<const f32x4 *>(sin_r + c0 / 2);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float a = f[2 * i], b = f[2 * i + 1];
+            f[2 * i] = __fsub_rn(__fmul_rn(a, c[i]), __fmul_rn(b, s[i]));
+            f[2 * i + 1] = __fadd_rn(__fmul_rn(b, c[i]), __fmul_rn(a, s[i]));
+        }
+    } else {
+        const int half = rot >> 1;
+        const bool low = c0 < half;
+        float o[8];
+        load8f(head + (low ? c0 + half : c0 - half), o);
+        const int r0 = low ? c0 : c0 - half;
+        float c[8], s[8];
+        *reinterpret_cast<f32x4 *>(c) = *reinterpret_cast<const f32x4 *>(cos_r + r0);
+        *reinterpret_cast<f32x4 *>(c + 4) = *reinterpret_cast<const f32x4 *>(cos_r + r0 + 4);
+        *reinterpret_cast<f32x4 *>(s) = *reinterpret_cast<const f32x4 *>(sin_r + r0);
+        *reinterpret_cast<f32x4 *>(s + 4) = *reinterpret_cast<const f32x4 *>(sin_r + r0 + 4);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            f[i] = low ? __fsub_rn(__fmul_rn(f[i], c[i]), __fmul_rn(o[i], s[i])) : __fadd_rn(__fmul_rn(f[i], c[i]), __fmul_rn(o[i], s[i]));
+    }
+}
+
+__device__ __forceinline__ unsigned to_codes4(float a, float b, float c, float d)
+{
+    // infinities saturate (the conversion would make them NaN); NaN stays NaN
+    const auto sat = [](float x) { return x > E4M3_MAX ? E4M3_MAX : (x < -E4M3_MAX ? -E4M3_MAX : x); };
+    int r = __builtin_amdgcn_cvt_pk_fp8_f32(sat(a), sat(b), 0, false);
+    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(sat(c), sat(d), r, true);
+}
+
+__device__ __forceinline__ unsigned scale_codes4(unsigned w, float f)
+{
+    return to_codes4(__builtin_amdgcn_cvt_f32_fp8(w, 0) * f, __builtin_amdgcn_cvt_f32_fp8(w, 1) * f, __builtin_amdgcn_cvt_f32_fp8(w, 2) * f,
+                     __builtin_amdgcn_cvt_f32_fp8(w, 3) * f);
+}
+
+__device__ __forceinline__ float pow2f(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }
+
+// the smallest e with a 2^-e <= 448 = 1.75 * 2^8, for the bits of a finite a >= 0
+__device__ __forceinline__ int exponent_for(unsigned bits)
+{
+    const int e = (int)(bits >> 23) - 135 + ((bits & 0x7fffff) > 0x600000);
+    return e < MIN_EXP ? MIN_EXP : (e > MAX_EXP ? MAX_EXP : e);
+}
+
+// The sequence that `pos` of a rising row of batch + 1 starts lies in: the last b < batch with f(b) <= pos.
+template <typename F>
+__device__ __forceinline__ int find_sequence(int batch, int64_t pos, F f)
+{
+    int lo = 0, hi = batch - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (f(mid) <= pos) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+template <typename T>
+__device__ __forceinline__ void append_page(const AppendArgs &a, int item, int head, bool is_v, unsigned *sm_max)
+{
+    const int tid = threadIdx.x, nt = blockDim.x;
+    int b = item, j = 0;
+    int64_t row0 = item, n = 1;
+    if (a.cu) {
+        // sequence b starts at item cu[b] / page + 2 b: room for the (n + page - 2) / page + 1 pages it can touch
+        const auto start = [&](int s) { return (int64_t)a.cu[s] / a.page + 2 * (int64_t)s; };
+        b = find_sequence(a.batch, item, start);
+        j = (int)(item - start(b));
+        row0 = a.cu[b];
+        n = (int64_t)a.cu[b + 1] - row0;
+        if (j < 0 || row0 < 0 || n <= 0 || row0 + n > a.n_tokens) return;
+    }
+    const int64_t past = a.past[b];
+    if (past < 0) return;
+    const int64_t pidx = past / a.page + j, first = pidx * a.page;   // the page's place in its sequence, its first position
+    int64_t end = past + n;
+    if (a.rot && end > a.max_pos) end = a.max_pos;   // positions without an angle are not stored
+    const int s0 = (int)(past > first ? past - first : 0);
+    const int s1 = (int)(end - first < a.page ? end - first : a.page);
+    if (s1 <= s0 || pidx >= a.table_width) return;
+    const int64_t page_id = a.table[(int64_t)b * a.table_width + pidx];
+    if (page_id < 0 || page_id >= a.n_pages) return;
+
+    const int d = a.head_dim, n_ch = d >> 3;
+    const T *x = is_v ? (const T *)a.v + head * a.v_head : (const T *)a.k + head * a.k_head;
+    const int64_t tok_stride = is_v ? a.v_tok : a.k_tok;
+    const int64_t block = page_id * a.n_kv_heads + head;
+    uint8_t *codes = (is_v ? a.v_codes : a.k_codes) + block * a.page * d;
+    float *scale = (is_v ? a.v_scale : a.k_scale) + block;
+    const float old = *scale;
+    const int64_t row_of_0 = row0 + first - past;   // row of the page's slot 0, were it new
+    // items that hold new tokens: quads s0 / 4 .. (s1 - 1) / 4
+    const int quad0 = s0 >> 2, live_quads = ((s1 - 1) >> 2) - quad0 + 1, n_live = live_quads * n_ch;
+
+    float f[4][8];
+    int quad = 0, ch = 0;
+    const auto fetch = [&](int it) {
+        // channels vary fastest for keys (a row is stored whole), tokens for values
+        quad = quad0 + (is_v ? it % live_quads : it / n_ch);
+        ch = is_v ? it / live_quads : it % n_ch;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const int s = 4 * quad + t;
+            if (s < s0 || s >= s1) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) f[t][i] = 0.f;
+                continue;
+            }
+            const T *p = x + (row_of_0 + s) * tok_stride;
+            if (is_v || a.rot == 0) load8f(p + 8 * ch, f[t]);
+            else load8_rotated(p, 8 * ch, a.cos_t + (first + s) * (a.rot >> 1), a.sin_t + (first + s) * (a.rot >> 1), a.rot, a.interleaved, f[t]);
+        }
+    };
+    unsigned most = 0;
+    for (int it = tid; it < n_live; it += nt) {
+        fetch(it);
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const unsigned bits = __float_as_uint(f[t][i]) & 0x7fffffffu;
+                if (bits < 0x7f800000u && bits > most) most = bits;
+            }
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+        const unsigned o = __shfl_xor(most, off, 64);
+        most = o > most ? o : most;
+    }
+    if (nt > 64) {
+        if ((tid & 63) == 0) sm_max[tid >> 6] = most;
+        __syncthreads();
+        for (int w = 0; w < nt >> 6; ++w) most = sm_max[w] > most ? sm_max[w] : most;
+    }
+    int e = exponent_for(most);
+    if (s0 > 0) {
+        // the tokens already there keep the scale from falling; a scale that is no power of two is rounded up to one
+        const unsigned ob = __float_as_uint(old);
+        int eo = old > 0.f && old < INFINITY ? (int)(ob >> 23) - 127 + ((ob & 0x7fffff) != 0) : MIN_EXP;
+        eo = eo < MIN_EXP ? MIN_EXP : (eo > MAX_EXP ? MAX_EXP : eo);
+        e = eo > e ? eo : e;
+        const float ratio = old > 0.f && old < INFINITY ? old * pow2f(-e) : 0.f;
+        if (ratio != 1.f) {
+            if (is_v) {
+                const int words = (s0 + 3) >> 2;
+                for (int i = tid; i < d * words; i += nt) {
+                    const int row = i / words, w = i - row * words;
+                    unsigned *p = reinterpret_cast<unsigned *>(codes + row * a.page) + w;
+                    const unsigned was = *p;
+                    const int kept = s0 - 4 * w;   // of the word's four tokens
+                    const unsigned mask = kept >= 4 ? 0xffffffffu : ((1u << (8 * kept)) - 1);
+                    *p = (scale_codes4(was, ratio) & mask) | (was & ~mask);
+                }
+            } else {
+                for (int i = tid; i < s0 * (d >> 2); i += nt) {
+                    unsigned *p = reinterpret_cast<unsigned *>(codes) + i;
+                    *p = scale_codes4(*p, ratio);
+                }
+            }
+            __syncthreads();   // a word of values may hold tokens of both kinds
+        }
+    }
+    if (tid == 0) *scale = pow2f(e);
+    const float inv = pow2f(-e);
+    for (int it = tid; it < n_live; it += nt) {
+        if (n_live > nt) fetch(it);
+        if (is_v) {
+            const bool whole = 4 * quad >= s0 && 4 * quad + 4 <= s1;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const unsigned w = to_codes4(f[0][i] * inv, f[1][i] * inv, f[2][i] * inv, f[3][i] * inv);
+                uint8_t *p = codes + (8 * ch + i) * a.page + 4 * quad;
+                if (whole) {
+                    *reinterpret_cast<unsigned *>(p) = w;
+                } else {
+#pragma unroll
+                    for (int t = 0; t < 4; ++t)
+                        if (4 * quad + t >= s0 && 4 * quad + t < s1) p[t] = (uint8_t)(w >> (8 * t));
+                }
+            }
+        } else {
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const int s = 4 * quad + t;
+                if (s < s0 || s >= s1) continue;
+                u32x2 w;
+                w[0] = to_codes4(f[t][0] * inv, f[t][1] * inv, f[t][2] * inv, f[t][3] * inv);
+                w[1] = to_codes4(f[t][4] * inv, f[t][5] * inv, f[t][6] * inv, f[t][7] * inv);
+                *reinterpret_cast<u32x2 *>(codes + s * d + 8 * ch) = w;
+            }
+        }
+    }
+}
+
+// The query rows of one token, a block of heads: a thread takes 8 channels and, where those are the lower half of a
+// rotated pair, their partners too, so that q_out may be q.
+template <typename T>
+__device__ __forceinline__ void rotate_query(const AppendArgs &a, int64_t token, int head_block)
+{
+    const int n_ch = a.head_dim >> 3, per = blockDim.x / n_ch;
+    const int hl = threadIdx.x / n_ch, ch = threadIdx.x - hl * n_ch, head = head_block * per + hl;
+    if (hl >= per || head >= a.n_heads) return;
+    int64_t pos;
+    if (a.cu) {
+        if (token < a.cu[0] || token >= a.cu[a.batch]) return;   // behind the last sequence: left as it is
+        const int b = find_sequence(a.batch, token, [&](int s) { return (int64_t)a.cu[s]; });
+        pos = a.past[b] < 0 ? -1 : (int64_t)a.past[b] + (token - a.cu[b]);
+    } else {
+        pos = a.past[token];
+    }
+    const T *x = (const T *)a.q + token * a.q_tok + head * a.q_head;
+    T *y = (T *)a.q_out + token * a.qo_tok + head * a.qo_head;
+    const bool known = pos >= 0 && pos < a.max_pos;
+    const int half = a.rot >> 1, c0 = 8 * ch;
+    const float *cr = a.cos_t + (known ? pos : 0) * half, *sr = a.sin_t + (known ? pos : 0) * half;
+    const bool pair = !a.interleaved && c0 < a.rot;
+    if (pair && c0 >= half) return;   // written with its partner
+    float lo[8], hi[8];
+    load8_rotated(x, c0, cr, sr, a.rot, a.interleaved, lo);
+    if (pair) load8_rotated(x, c0 + half, cr, sr, a.rot, 0, hi);
+    if (!known) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) lo[i] = hi[i] = NAN;
+    }
+    store8f(y + c0, lo);
+    if (pair) store8f(y + c0 + half, hi);
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void kv_append_kernel(const AppendArgs a)
+{
+    __shared__ unsigned sm_max[4];
+    const unsigned n_kv = (unsigned)a.n_items * a.n_kv_heads * 2;
+    if (blockIdx.x < n_kv) {
+        const unsigned ih = blockIdx.x >> 1, item = ih / a.n_kv_heads;
+        append_page<T>(a, (int)item, (int)(ih - item * a.n_kv_heads), blockIdx.x & 1, sm_max);
+    } else {
+        const int per = blockDim.x / (a.head_dim >> 3);
+        const unsigned blocks = (a.n_heads + per - 1) / per, i = blockIdx.x - n_kv;
+        rotate_query<T>(a, i / blocks, (int)(i % blocks));
+    }
+}
+
+}  // namespace
+
+extern "C" int gq_kv_append(void *k_codes, void *v_codes, float *k_scale, float *v_scale, int64_t n_pages, int n_kv_heads, int page,
+                            int head_dim, const void *k, int64_t k_token_stride, int64_t k_head_stride, const void *v, int64_t v_token_stride,
+                            int64_t v_head_stride, int dtype, int64_t n_tokens, const int32_t *block_table, int64_t table_width,
+                            const int32_t *past_lens, const int32_t *cu_seqlens, int64_t batch, const void *q, int64_t q_token_stride,
+                            int64_t q_head_stride, int n_heads, void *q_out, int64_t q_out_token_stride, int64_t q_out_head_stride,
+                            const float *cos_t, const float *sin_t, int64_t max_pos, int rotary_dim, int interleaved, gq_stream_t stream)
+{
+    GQ_REQUIRE(dtype == GQ_F16 || dtype == GQ_BF16, "gq_kv_append: dtype %d is neither fp16 (0) nor bf16 (1)", dtype);
+    GQ_REQUIRE(head_dim >= 16 && head_dim <= 128 && head_dim % 16 == 0, "gq_kv_append: head_dim %d is not a multiple of 16 up to 128", head_dim);
+    GQ_REQUIRE(page == 16 || page == 32 || page == 64 || page == 128, "gq_kv_append: pages of %d tokens: 16, 32, 64 or 128 are supported", page);
+    GQ_REQUIRE(n_kv_heads > 0 && n_pages >= 0 && n_tokens >= 0 && batch >= 0 && table_width >= 0, "gq_kv_append: negative size");
+    GQ_REQUIRE(batch < (1 << 24) && n_tokens < ((int64_t)1 << 31) && n_kv_heads <= 65536 && n_heads <= 65536, "gq_kv_append: too many tokens, sequences or heads");
+    GQ_REQUIRE(cu_seqlens || n_tokens == batch, "gq_kv_append: %lld tokens for %lld sequences need cu_seqlens", (long long)n_tokens, (long long)batch);
+    GQ_REQUIRE(rotary_dim >= 0 && rotary_dim <= head_dim && rotary_dim % 16 == 0, "gq_kv_append: rotary_dim %d is not a multiple of 16 up to head_dim", rotary_dim);
+    if (n_tokens == 0 || batch == 0) return GQ_OK;
+    GQ_REQUIRE(k_codes && v_codes && k_scale && v_scale && k && v && block_table && past_lens, "gq_kv_append: NULL pointer");
+    GQ_REQUIRE(!rotary_dim || (cos_t && sin_t && max_pos > 0), "gq_kv_append: a rotation needs the tables of cosines and sines");
+    GQ_REQUIRE(!q || (q_out && n_heads > 0 && rotary_dim), "gq_kv_append: q needs an output, heads and a rotation");
+    GQ_REQUIRE(k_token_stride % 8 == 0 && k_head_stride % 8 == 0 && v_token_stride % 8 == 0 && v_head_stride % 8 == 0 &&
+                   (!q || (q_token_stride % 8 == 0 && q_head_stride % 8 == 0 && q_out_token_stride % 8 == 0 && q_out_head_stride % 8 == 0)),
+               "gq_kv_append: strides must be multiples of 8 elements");
+    GQ_REQUIRE((((uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q | (uintptr_t)q_out | (uintptr_t)cos_t |
+                 (uintptr_t)sin_t) & 15) == 0, "gq_kv_append: pointers must be 16-byte aligned");
+    AppendArgs a;
+    a.q = q, a.k = k, a.v = v, a.q_out = q_out;
+    a.q_tok = q_token_stride, a.q_head = q_head_stride, a.qo_tok = q_out_token_stride, a.qo_head = q_out_head_stride;
+    a.k_tok = k_token_stride, a.k_head = k_head_stride, a.v_tok = v_token_stride, a.v_head = v_head_stride;
+    a.k_codes = (uint8_t *)k_codes, a.v_codes = (uint8_t *)v_codes, a.k_scale = k_scale, a.v_scale = v_scale;
+    a.cos_t = cos_t, a.sin_t = sin_t, a.table = block_table, a.past = past_lens, a.cu = cu_seqlens;
+    a.n_tokens = n_tokens, a.max_pos = max_pos, a.n_pages = n_pages, a.table_width = table_width;
+    a.batch = (int)batch, a.n_heads = n_heads, a.n_kv_heads = n_kv_heads, a.head_dim = head_dim, a.page = page;
+    a.rot = rotary_dim, a.interleaved = interleaved != 0;
+    const int64_t n_items = cu_seqlens ? n_tokens / page + 2 * batch : batch;
+    // one wave where a workgroup has a single token (or a small page) to look after
+    const int items_per_page = (cu_seqlens ? page / 4 : 1) * (head_dim / 8);
+    const int threads = items_per_page <= 64 ? 64 : (items_per_page <= 128 ? 128 : 256);
+    const int64_t q_blocks = q ? n_tokens * gq_cdiv(n_heads, threads / (head_dim / 8)) : 0;
+    const int64_t grid = n_items * n_kv_heads * 2 + q_blocks;
+    GQ_REQUIRE(grid < ((int64_t)1 << 31), "gq_kv_append: too many tokens for one call");
+    a.n_items = (int)n_items;
+    if (dtype == GQ_F16) hipLaunchKernelGGL(kv_append_kernel<_Float16>, dim3((unsigned)grid), dim3(threads), 0, (hipStream_t)stream, a);
+    else hipLaunchKernelGGL(kv_append_kernel<__bf16>, dim3((unsigned)grid), dim3(threads), 0, (hipStream_t)stream, a);
+    GQ_LAUNCH_CHECK();
+    return GQ_OK;
+}

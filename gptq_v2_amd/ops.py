@@ -6,7 +6,7 @@ PyTorch is used for device memory and streams only; every function validates its
 from __future__ import annotations
 
 import ctypes
-from typing import Optional, Sequence, Tuple
+from typing import NamedTuple, Optional, Sequence, Tuple
 
 import torch
 
@@ -580,3 +580,225 @@ def gemm_nt(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
         rc = _lib.load().gq_gemm_nt(_p(y), _p(x), _p(weight), m, n, k, code, _stream(x))
     _lib.check(rc, "gq_gemm_nt")
     return y
+
+
+# ---- serving a quantised decoder --------------------------------------------------------------------------------
+
+class PagedCache(NamedTuple):
+    """Keys and values in pages of 16, 32, 64 or 128 tokens: e4m3 codes (``torch.float8_e4m3fn``) and one fp32 scale per
+    (page, kv head); value = code * scale.  Values lie by channel, (pages, heads, head_dim, tokens): the attention reads
+    them as an operand whose inner index is the token."""
+    k: torch.Tensor         # (pages, kv heads, page, head_dim)
+    v: torch.Tensor         # (pages, kv heads, head_dim, page)
+    k_scale: torch.Tensor   # (pages, kv heads)
+    v_scale: torch.Tensor   # (pages, kv heads)
+
+    @classmethod
+    def empty(cls, n_pages: int, n_kv_heads: int, page: int, head_dim: int, device) -> "PagedCache":
+        """A pool of pages that hold zeros."""
+        code = dict(dtype=torch.float8_e4m3fn, device=device)
+        return cls(torch.zeros(n_pages, n_kv_heads, page, head_dim, **code), torch.zeros(n_pages, n_kv_heads, head_dim, page, **code),
+                   torch.ones(n_pages, n_kv_heads, device=device), torch.ones(n_pages, n_kv_heads, device=device))
+
+
+class TokenLogprobs(NamedTuple):
+    logprob: torch.Tensor                  # (rows...) fp32
+    entropy: torch.Tensor                  # (rows...) fp32, nats
+    top_logprob: Optional[torch.Tensor]    # (rows..., top) fp32
+    top_token: Optional[torch.Tensor]      # (rows..., top) int64
+
+
+def _no_grad(*ts: Optional[torch.Tensor]) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+        raise RuntimeError("this operator has no backward pass: call it under torch.no_grad() or on detached tensors")
+
+
+def _rows(t: torch.Tensor, name: str, like: Optional[torch.Tensor] = None) -> None:
+    """A (tokens, heads, head_dim) tensor whose last dimension is dense; the others may have any stride of 8 elements."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: expected a tensor")
+    if t.device.type != "cuda":
+        raise ValueError(f"{name}: must live on the GPU (got {t.device}); there is no CPU path")
+    if t.dim() != 3:
+        raise ValueError(f"{name}: expected (tokens, heads, head_dim), got {t.dim()} dimensions")
+    if t.shape[2] > 1 and t.stride(2) != 1:
+        raise ValueError(f"{name}: the last dimension must be contiguous")
+    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+        raise ValueError(f"{name}: is {t.dtype} on {t.device}, expected {like.dtype} on {like.device}")
+
+
+def _ints(t: torch.Tensor, name: str, shape: Tuple[int, ...], device) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: expected a tensor")
+    if t.dtype != torch.int32 or t.device != device or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name}: expected contiguous int32 {shape} on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+
+
+def _check_cache(cache: PagedCache, device) -> Tuple[int, int, int, int]:
+    for t, name in zip(cache, PagedCache._fields):
+        _check(t, name, torch.float32 if name.endswith("scale") else torch.float8_e4m3fn, 2 if name.endswith("scale") else 4)
+        if t.device != device:
+            raise ValueError(f"{name}: on {t.device}, expected {device}")
+    n_pages, heads, page, d = cache.k.shape
+    if cache.v.shape != (n_pages, heads, d, page) or cache.k_scale.shape != (n_pages, heads) or cache.v_scale.shape != (n_pages, heads):
+        raise ValueError(f"the cache's tensors do not belong together: {[tuple(t.shape) for t in cache]}")
+    return n_pages, heads, page, d
+
+
+def _of(t: Optional[torch.Tensor]):
+    """pointer, token stride, head stride"""
+    return (t.data_ptr(), t.stride(0), t.stride(1)) if t is not None else (None, 0, 0)
+
+
+def _out_like(out: Optional[torch.Tensor], q: torch.Tensor) -> torch.Tensor:
+    if out is None:
+        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    _rows(out, "out", q)
+    if out.shape != q.shape:
+        raise ValueError(f"out is {tuple(out.shape)}, q {tuple(q.shape)}")
+    return out
+
+
+def attention_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None, causal: bool = True,
+                     scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention over whole prompts: q (tokens, heads, head_dim), k / v (tokens, kv heads, head_dim) in fp16 or bf16, head_dim
+    a multiple of 8 up to 128; strided views (slices of a merged q/k/v product) are taken as they are.  ``cu_seqlens``
+    (sequences + 1) int32 says where the packed sequences begin and end (None: one sequence); rows behind the last are left
+    as they are.  Causal: token i of a sequence sees tokens 0..i.  ``scale`` defaults to head_dim ** -0.5."""
+    _no_grad(q, k, v, out)
+    _rows(q, "q")
+    _rows(k, "k", q)
+    _rows(v, "v", q)
+    code = _dtype_code(q)
+    t, heads, d = q.shape
+    if k.shape != v.shape or k.shape[0] != t or k.shape[2] != d or k.shape[1] == 0 or heads % k.shape[1]:
+        raise ValueError(f"q is {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
+    batch = 1
+    if cu_seqlens is not None:
+        batch = cu_seqlens.shape[0] - 1 if isinstance(cu_seqlens, torch.Tensor) and cu_seqlens.dim() == 1 else 0
+        _ints(cu_seqlens, "cu_seqlens", (batch + 1,), q.device)
+    out = _out_like(out, q)
+    with torch.cuda.device(q.device):
+        rc = _lib.load().gq_attention_prompt(*_of(out), *_of(q), *_of(k), *_of(v), code, t, heads, k.shape[1], d, _p(cu_seqlens), batch,
+                                             int(causal), float(d ** -0.5 if scale is None else scale), _stream(q))
+    _lib.check(rc, "gq_attention_prompt")
+    return out
+
+
+def kv_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor, past_lens: torch.Tensor,
+              cu_seqlens: Optional[torch.Tensor] = None, q: Optional[torch.Tensor] = None, cos: Optional[torch.Tensor] = None,
+              sin: Optional[torch.Tensor] = None, interleaved: bool = False, q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """Appends the new tokens' keys and values, k / v (tokens, kv heads, head_dim) in fp16 or bf16, to the cache, behind the
+    ``past_lens`` (sequences) int32 tokens that each sequence has; ``block_table`` (sequences, width) int32 names its pages.
+    ``cu_seqlens`` None: one new token for each sequence.  With ``cos`` / ``sin`` (positions, rotary_dim / 2) fp32 the keys are
+    rotated on the way, and q (tokens, heads, head_dim), if given, into ``q_out`` (which may be q), which is returned; pairs of
+    channels are (j, j + rotary_dim / 2), or (2j, 2j + 1) if ``interleaved``.  See gq_kv_append in gptq_amd.h for the scales
+    and for tokens without a page or an angle."""
+    _no_grad(k, v, q)
+    _rows(k, "k")
+    _rows(v, "v", k)
+    code = _dtype_code(k)
+    n_pages, heads, page, d = _check_cache(cache, k.device)
+    t = k.shape[0]
+    if k.shape != v.shape or k.shape[1:] != (heads, d):
+        raise ValueError(f"k is {tuple(k.shape)}, v {tuple(v.shape)}, the cache has {heads} heads of {d}")
+    if not isinstance(block_table, torch.Tensor) or block_table.dim() != 2:
+        raise ValueError("block_table: expected (sequences, pages)")
+    batch, width = block_table.shape
+    _ints(block_table, "block_table", (batch, width), k.device)
+    _ints(past_lens, "past_lens", (batch,), k.device)
+    if cu_seqlens is not None:
+        _ints(cu_seqlens, "cu_seqlens", (batch + 1,), k.device)
+    elif t != batch:
+        raise ValueError(f"{t} tokens for {batch} sequences need cu_seqlens")
+    rot = max_pos = 0
+    if (cos is None) != (sin is None):
+        raise ValueError("cos and sin belong together")
+    if cos is not None:
+        _check(cos, "cos", torch.float32, 2)
+        _check(sin, "sin", torch.float32, 2)
+        if cos.shape != sin.shape or cos.device != k.device or sin.device != k.device:
+            raise ValueError(f"cos is {tuple(cos.shape)} on {cos.device}, sin {tuple(sin.shape)} on {sin.device}")
+        max_pos, rot = cos.shape[0], 2 * cos.shape[1]
+    n_heads = 0
+    if q is not None:
+        if not rot:
+            raise ValueError("q is given to be rotated: cos and sin are missing")
+        _rows(q, "q", k)
+        if q.shape[0] != t or q.shape[2] != d:
+            raise ValueError(f"q is {tuple(q.shape)}, k {tuple(k.shape)}")
+        n_heads = q.shape[1]
+        q_out = _out_like(q_out, q)
+    elif q_out is not None:
+        raise ValueError("q_out without q")
+    with torch.cuda.device(k.device):
+        rc = _lib.load().gq_kv_append(cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), n_pages, heads, page,
+                                      d, *_of(k), *_of(v), code, t, block_table.data_ptr(), width, past_lens.data_ptr(), _p(cu_seqlens), batch,
+                                      *_of(q), n_heads, *_of(q_out), _p(cos), _p(sin), max_pos, rot, int(interleaved), _stream(k))
+    _lib.check(rc, "gq_kv_append")
+    return q_out
+
+
+def attention_paged(q: torch.Tensor, cache: PagedCache, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                    cu_seqlens: Optional[torch.Tensor] = None, scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of q (tokens, heads, head_dim) in fp16 or bf16 over the cached tokens of each sequence, ``seq_lens``
+    (sequences) int32 of them with the query tokens included: its n query tokens are its last n, each sees the keys up to its
+    own position.  ``cu_seqlens`` None: one query token for each sequence (a decoder's step); several are a checked
+    draft or a chunk of a prompt behind its cached beginning.  A row that sees nothing is 0; a sequence with a token on no page
+    is NaN.  The scratch memory of long sequences comes from torch's allocator, a tensor per call."""
+    _no_grad(q, out)
+    _rows(q, "q")
+    code = _dtype_code(q)
+    n_pages, kv_heads, page, d = _check_cache(cache, q.device)
+    t, heads, dq = q.shape
+    if dq != d or kv_heads == 0 or heads % kv_heads:
+        raise ValueError(f"q is {tuple(q.shape)}, the cache has {kv_heads} heads of {d}")
+    if not isinstance(block_table, torch.Tensor) or block_table.dim() != 2:
+        raise ValueError("block_table: expected (sequences, pages)")
+    batch, width = block_table.shape
+    _ints(block_table, "block_table", (batch, width), q.device)
+    _ints(seq_lens, "seq_lens", (batch,), q.device)
+    if cu_seqlens is not None:
+        _ints(cu_seqlens, "cu_seqlens", (batch + 1,), q.device)
+    elif t != batch:
+        raise ValueError(f"{t} query tokens for {batch} sequences need cu_seqlens")
+    out = _out_like(out, q)
+    lib = _lib.load()
+    with torch.cuda.device(q.device):
+        need = lib.gq_attention_paged_workspace(t, batch, int(cu_seqlens is not None), heads, kv_heads, d, page, width)
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        rc = lib.gq_attention_paged(*_of(out), *_of(q), code, t, heads, cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
+                                    cache.v_scale.data_ptr(), n_pages, kv_heads, page, d, block_table.data_ptr(), width, seq_lens.data_ptr(),
+                                    _p(cu_seqlens), batch, float(d ** -0.5 if scale is None else scale), _p(ws), need, _stream(q))
+    _lib.check(rc, "gq_attention_paged")
+    return out
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, ignore_index: int = -100) -> TokenLogprobs:
+    """Log probabilities of ``tokens`` (rows...) int64 under ``logits`` (rows..., vocab) in fp16, bf16 or fp32, with each row's
+    entropy and its ``top`` (0..32) most likely words, ties to the lowest index; everything in fp32 from one read of the
+    logits.  Logits of any row stride are taken as they are (a slice of sequences without their last token is copied).
+    A token equal to ``ignore_index`` gives 0, any other that is no word NaN; -inf is a word that cannot come."""
+    _no_grad(logits)
+    if not isinstance(logits, torch.Tensor) or not isinstance(tokens, torch.Tensor):
+        raise TypeError("logits and tokens: expected tensors")
+    if logits.device.type != "cuda":
+        raise ValueError(f"logits: must live on the GPU (got {logits.device}); there is no CPU path")
+    code = 2 if logits.dtype == torch.float32 else _dtype_code(logits)
+    if logits.dim() == 0 or tokens.shape != logits.shape[:-1] or tokens.dtype != torch.int64 or tokens.device != logits.device:
+        raise ValueError(f"logits are {tuple(logits.shape)} on {logits.device}, tokens {tokens.dtype} {tuple(tokens.shape)} on {tokens.device}")
+    vocab = logits.shape[-1]
+    rows = logits if logits.dim() == 2 else logits.reshape(-1, vocab) if vocab else logits.reshape(0, 0)
+    if rows.numel() and (rows.stride(1) != 1 and vocab > 1 or rows.stride(0) < vocab):
+        rows = rows.contiguous()
+    n, dev, shape = tokens.numel(), logits.device, tuple(tokens.shape)
+    flat = tokens.reshape(-1).contiguous()
+    lp = torch.empty(shape, dtype=torch.float32, device=dev)
+    ent = torch.empty(shape, dtype=torch.float32, device=dev)
+    tlp = torch.empty(*shape, top, dtype=torch.float32, device=dev) if top > 0 else None
+    tok = torch.empty(*shape, top, dtype=torch.int64, device=dev) if top > 0 else None
+    with torch.cuda.device(dev):
+        rc = _lib.load().gq_token_logprobs(_p(rows), code, n, rows.stride(0) if n else vocab, vocab, _p(flat), int(ignore_index), _p(lp), _p(ent),
+                                           int(top), _p(tlp), _p(tok), _stream(logits))
+    _lib.check(rc, "gq_token_logprobs")
+    return TokenLogprobs(lp, ent, tlp, tok)

@@ -10,7 +10,7 @@
  *     asynchronous with respect to the host unless stated otherwise;
  *   - return value: 0 on success, a negative GQ_E* code on error; gq_last_error()
  *     returns a thread-local, human-readable description of the last failure;
- *   - dtype codes: GQ_F16 = 0 (IEEE binary16), GQ_BF16 = 1;
+ *   - dtype codes: GQ_F16 = 0 (IEEE binary16), GQ_BF16 = 1, GQ_F32 = 2 where an entry point says so;
  *   - a tensor with zero rows may be passed as NULL (an empty torch tensor has no data
  *     pointer): gq_xtx_accumulate with n_tokens == 0, gq_permute_columns and the W4A16
  *     GEMMs with m == 0 return 0 without a launch.
@@ -30,6 +30,7 @@ extern "C" {
 
 #define GQ_F16 0
 #define GQ_BF16 1
+#define GQ_F32 2 /* gq_token_logprobs only */
 
 #define GQ_OK 0
 #define GQ_EINVAL (-1)     /* bad argument (shape, dtype code, alignment, NULL) */
@@ -400,6 +401,67 @@ int gq_silu_mul(void *out, const void *gate, const void *up, int dtype, int64_t 
  *      the stage-wise replay of gptq_v2_amd.driver.quantize_llama. */
 int gq_rope_inplace(void *x, int64_t row_stride, const void *cos_t, const void *sin_t, int64_t cs_batch_stride, int64_t n_batch,
                     int64_t seq, int n_heads, int head_dim, int dtype, gq_stream_t stream);
+
+/* ---- serving a quantised decoder (no reference counterpart: the reference stops at the reconstructed weights) ----
+ *
+ * Sequences are packed: row i of a [n_tokens][heads][head_dim] tensor belongs to the sequence b with
+ * cu_seqlens[b] <= i < cu_seqlens[b + 1] (int32, batch + 1 of them, rising).  Rows behind cu_seqlens[batch] are neither
+ * read nor written.  Such tensors are given by a token and a head stride in elements (multiples of 8, 16-byte aligned
+ * pointers), so that q, k and v may be slices of one merged product.  Query head h reads kv head h / (n_heads / n_kv_heads).
+ *
+ * gq_attention_prompt: out = softmax(softmax_scale q k^T) v within each sequence; causal != 0: query i sees keys 0..i.
+ * cu_seqlens NULL: one sequence of n_tokens (batch 1).  head_dim a multiple of 8 up to 128, sums and softmax in fp32, the
+ * weights rounded to `dtype` for the second product. */
+int gq_attention_prompt(void *out, int64_t out_token_stride, int64_t out_head_stride, const void *q, int64_t q_token_stride,
+                        int64_t q_head_stride, const void *k, int64_t k_token_stride, int64_t k_head_stride, const void *v,
+                        int64_t v_token_stride, int64_t v_head_stride, int dtype, int64_t n_tokens, int n_heads, int n_kv_heads,
+                        int head_dim, const int32_t *cu_seqlens, int64_t batch, int causal, float softmax_scale, gq_stream_t stream);
+
+/* A paged cache of keys and values in 8 bits: e4m3 (OCP) codes with one scale per (page, kv head) and tensor,
+ *   k_codes[n_pages][n_kv_heads][page][head_dim], v_codes[n_pages][n_kv_heads][head_dim][page]  (values by channel),
+ *   k_scale, v_scale[n_pages][n_kv_heads] fp32;  value = code * scale.
+ * page is 16, 32, 64 or 128 tokens, head_dim a multiple of 16 up to 128.  block_table[batch][table_width] names the pages
+ * of each sequence in order; an entry outside 0..n_pages-1 is no page.
+ *
+ * gq_kv_append writes the new tokens of each sequence behind the past_lens[b] it has: the keys rotated, both in e4m3
+ * at the page's scale, 2^e with the smallest e (at least -100) for which the page's finite magnitudes fit 448 2^e.  When a
+ * page already holds tokens of the sequence its scale does not fall, and they are re-expressed when it grows.  Infinities
+ * saturate, NaN stays NaN.  Slots behind the new tokens stay as they are.  No page may be appended to by two sequences of a call.
+ * cu_seqlens NULL: one new token per sequence (n_tokens == batch).
+ * Rotation of the first rotary_dim channels (a multiple of 16; 0: none) by position p = past_lens[b] + i with
+ * cos / sin [max_pos][rotary_dim / 2] fp32: channel pairs (j, j + rotary_dim / 2), or (2j, 2j + 1) if interleaved,
+ *   a' = a cos - b sin,  b' = b cos + a sin,  each operation rounded to fp32.
+ * q (may be NULL) is rotated the same way into q_out (may be q), rounded once to `dtype`.
+ * A token on no page, or whose position has no row in the tables, is not stored; a query row without an angle is NaN.
+ * past_lens[b] < 0: nothing is stored for that sequence. */
+int gq_kv_append(void *k_codes, void *v_codes, float *k_scale, float *v_scale, int64_t n_pages, int n_kv_heads, int page,
+                 int head_dim, const void *k, int64_t k_token_stride, int64_t k_head_stride, const void *v, int64_t v_token_stride,
+                 int64_t v_head_stride, int dtype, int64_t n_tokens, const int32_t *block_table, int64_t table_width,
+                 const int32_t *past_lens, const int32_t *cu_seqlens, int64_t batch, const void *q, int64_t q_token_stride,
+                 int64_t q_head_stride, int n_heads, void *q_out, int64_t q_out_token_stride, int64_t q_out_head_stride,
+                 const float *cos_t, const float *sin_t, int64_t max_pos, int rotary_dim, int interleaved, gq_stream_t stream);
+
+/* Attention of each sequence's query tokens over its cached keys and values: the n query tokens of sequence b are the last
+ * n of its seq_lens[b], and each sees the keys up to its own position (a row that sees none is 0).  cu_seqlens NULL: one
+ * query token per sequence.  Any positive scales are taken; products in fp32, the weights rounded to fp16 for the second.
+ * A sequence with a token on no page, or longer than its table, comes out as NaN.
+ * gq_attention_paged_workspace: bytes of scratch memory a call of these sizes needs (0: none); ragged = cu_seqlens given. */
+size_t gq_attention_paged_workspace(int64_t n_tokens, int64_t batch, int ragged, int n_heads, int n_kv_heads, int head_dim, int page,
+                                    int64_t table_width);
+int gq_attention_paged(void *out, int64_t out_token_stride, int64_t out_head_stride, const void *q, int64_t q_token_stride,
+                       int64_t q_head_stride, int dtype, int64_t n_tokens, int n_heads, const void *k_codes, const void *v_codes,
+                       const float *k_scale, const float *v_scale, int64_t n_pages, int n_kv_heads, int page, int head_dim,
+                       const int32_t *block_table, int64_t table_width, const int32_t *seq_lens, const int32_t *cu_seqlens,
+                       int64_t batch, float softmax_scale, void *workspace, size_t workspace_bytes, gq_stream_t stream);
+
+/* Per row of logits[n_rows][row_stride] (dtype GQ_F16, GQ_BF16 or GQ_F32; vocab of them count): logprob[row], the log
+ * probability of tokens[row] (0 where that is ignore_index, NaN where it is no other word of the vocabulary); entropy[row]
+ * in nats; and the `top` (0..32) most likely words with their log probabilities, ties to the lowest index.  -inf is a word
+ * that cannot come; a row with NaN or +inf, or of -inf alone, gives NaN (its words are those a stable descending sort puts
+ * first).  Sums in fp32. */
+int gq_token_logprobs(const void *logits, int dtype, int64_t n_rows, int64_t row_stride, int64_t vocab, const int64_t *tokens,
+                      int64_t ignore_index, float *logprob, float *entropy, int top, float *top_logprob, int64_t *top_token,
+                      gq_stream_t stream);
 
 #ifdef __cplusplus
 }
