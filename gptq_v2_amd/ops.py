@@ -608,41 +608,76 @@ class TokenLogprobs(NamedTuple):
     top_token: Optional[torch.Tensor]      # (rows..., top) int64
 
 
+# A decoder's step calls these operators once per layer and token with little work each, so the checks first ask for what is
+# nearly always so, cheaply, and look for the reason only when it is not.
+
 def _no_grad(*ts: Optional[torch.Tensor]) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
-        raise RuntimeError("this operator has no backward pass: call it under torch.no_grad() or on detached tensors")
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                raise RuntimeError("this operator has no backward pass: call it under torch.no_grad() or on detached tensors")
 
 
 def _rows(t: torch.Tensor, name: str, like: Optional[torch.Tensor] = None) -> None:
     """A (tokens, heads, head_dim) tensor whose last dimension is dense; the others may have any stride of 8 elements."""
+    if isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 3 and t.stride(2) == 1 and (
+            like is None or t.dtype == like.dtype and t.get_device() == like.get_device()):
+        return
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: expected a tensor")
     if t.device.type != "cuda":
         raise ValueError(f"{name}: must live on the GPU (got {t.device}); there is no CPU path")
     if t.dim() != 3:
         raise ValueError(f"{name}: expected (tokens, heads, head_dim), got {t.dim()} dimensions")
-    if t.shape[2] > 1 and t.stride(2) != 1:
+    if t.stride(2) != 1:
         raise ValueError(f"{name}: the last dimension must be contiguous")
-    if like is not None and (t.dtype != like.dtype or t.device != like.device):
-        raise ValueError(f"{name}: is {t.dtype} on {t.device}, expected {like.dtype} on {like.device}")
+    raise ValueError(f"{name}: is {t.dtype} on {t.device}, expected {like.dtype} on {like.device}")
 
 
-def _ints(t: torch.Tensor, name: str, shape: Tuple[int, ...], device) -> None:
+def _ints(t: torch.Tensor, name: str, shape: Tuple[int, ...], like: torch.Tensor) -> None:
+    if isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.shape == shape and t.get_device() == like.get_device() and t.is_contiguous():
+        return
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: expected a tensor")
-    if t.dtype != torch.int32 or t.device != device or t.shape != shape or not t.is_contiguous():
-        raise ValueError(f"{name}: expected contiguous int32 {shape} on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    raise ValueError(f"{name}: expected contiguous int32 {shape} on {like.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
-def _check_cache(cache: PagedCache, device) -> Tuple[int, int, int, int]:
+def _check_cache(cache: PagedCache, like: torch.Tensor) -> Tuple[int, int, int, int]:
+    k, v, ks, vs = cache
+    dev = like.get_device()
+    if (isinstance(k, torch.Tensor) and isinstance(v, torch.Tensor) and isinstance(ks, torch.Tensor) and isinstance(vs, torch.Tensor)
+            and k.dtype is torch.float8_e4m3fn and v.dtype is torch.float8_e4m3fn and ks.dtype is torch.float32 and vs.dtype is torch.float32
+            and k.get_device() == dev and v.get_device() == dev and ks.get_device() == dev and vs.get_device() == dev and k.dim() == 4
+            and k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
+        n_pages, heads, page, d = k.shape
+        if v.shape == (n_pages, heads, d, page) and ks.shape == (n_pages, heads) and vs.shape == (n_pages, heads):
+            return n_pages, heads, page, d
     for t, name in zip(cache, PagedCache._fields):
         _check(t, name, torch.float32 if name.endswith("scale") else torch.float8_e4m3fn, 2 if name.endswith("scale") else 4)
-        if t.device != device:
-            raise ValueError(f"{name}: on {t.device}, expected {device}")
-    n_pages, heads, page, d = cache.k.shape
-    if cache.v.shape != (n_pages, heads, d, page) or cache.k_scale.shape != (n_pages, heads) or cache.v_scale.shape != (n_pages, heads):
-        raise ValueError(f"the cache's tensors do not belong together: {[tuple(t.shape) for t in cache]}")
-    return n_pages, heads, page, d
+        if t.get_device() != dev:
+            raise ValueError(f"{name}: on {t.device}, expected {like.device}")
+    raise ValueError(f"the cache's tensors do not belong together: {[tuple(t.shape) for t in cache]}")
+
+
+def _table(t: torch.Tensor, like: torch.Tensor) -> Tuple[int, int]:
+    if not isinstance(t, torch.Tensor) or t.dim() != 2:
+        raise ValueError("block_table: expected (sequences, pages)")
+    shape = t.shape
+    _ints(t, "block_table", shape, like)
+    return shape
+
+
+def _launch(name: str, like: torch.Tensor, *args) -> None:
+    """The C entry `name` on the device and current stream of `like`."""
+    fn = getattr(_lib.load(), name)
+    dev = like.get_device()
+    if torch._C._cuda_getDevice() == dev:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        _lib.check(rc, name)
 
 
 def _of(t: Optional[torch.Tensor]):
@@ -652,7 +687,7 @@ def _of(t: Optional[torch.Tensor]):
 
 def _out_like(out: Optional[torch.Tensor], q: torch.Tensor) -> torch.Tensor:
     if out is None:
-        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        return q.new_empty(q.shape)
     _rows(out, "out", q)
     if out.shape != q.shape:
         raise ValueError(f"out is {tuple(out.shape)}, q {tuple(q.shape)}")
@@ -671,17 +706,17 @@ def attention_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     _rows(v, "v", q)
     code = _dtype_code(q)
     t, heads, d = q.shape
-    if k.shape != v.shape or k.shape[0] != t or k.shape[2] != d or k.shape[1] == 0 or heads % k.shape[1]:
+    tk, kv_heads, dk = k.shape
+    if k.shape != v.shape or tk != t or dk != d or kv_heads == 0 or heads % kv_heads:
         raise ValueError(f"q is {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
-    batch = 1
+    batch, cu = 1, None
     if cu_seqlens is not None:
-        batch = cu_seqlens.shape[0] - 1 if isinstance(cu_seqlens, torch.Tensor) and cu_seqlens.dim() == 1 else 0
-        _ints(cu_seqlens, "cu_seqlens", (batch + 1,), q.device)
+        batch = cu_seqlens.numel() - 1 if isinstance(cu_seqlens, torch.Tensor) else 0
+        _ints(cu_seqlens, "cu_seqlens", (batch + 1,), q)
+        cu = cu_seqlens.data_ptr()
     out = _out_like(out, q)
-    with torch.cuda.device(q.device):
-        rc = _lib.load().gq_attention_prompt(*_of(out), *_of(q), *_of(k), *_of(v), code, t, heads, k.shape[1], d, _p(cu_seqlens), batch,
-                                             int(causal), float(d ** -0.5 if scale is None else scale), _stream(q))
-    _lib.check(rc, "gq_attention_prompt")
+    _launch("gq_attention_prompt", q, *_of(out), *_of(q), *_of(k), *_of(v), code, t, heads, kv_heads, d, cu, batch, causal,
+            d ** -0.5 if scale is None else scale)
     return out
 
 
@@ -694,21 +729,21 @@ def kv_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, block_table: 
     rotated on the way, and q (tokens, heads, head_dim), if given, into ``q_out`` (which may be q), which is returned; pairs of
     channels are (j, j + rotary_dim / 2), or (2j, 2j + 1) if ``interleaved``.  See gq_kv_append in gptq_amd.h for the scales
     and for tokens without a page or an angle."""
-    _no_grad(k, v, q)
+    _no_grad(k, v, q, q_out)
     _rows(k, "k")
     _rows(v, "v", k)
     code = _dtype_code(k)
-    n_pages, heads, page, d = _check_cache(cache, k.device)
-    t = k.shape[0]
-    if k.shape != v.shape or k.shape[1:] != (heads, d):
+    n_pages, heads, page, d = _check_cache(cache, k)
+    shape = k.shape
+    t = shape[0]
+    if shape != v.shape or shape != (t, heads, d):
         raise ValueError(f"k is {tuple(k.shape)}, v {tuple(v.shape)}, the cache has {heads} heads of {d}")
-    if not isinstance(block_table, torch.Tensor) or block_table.dim() != 2:
-        raise ValueError("block_table: expected (sequences, pages)")
-    batch, width = block_table.shape
-    _ints(block_table, "block_table", (batch, width), k.device)
-    _ints(past_lens, "past_lens", (batch,), k.device)
+    batch, width = _table(block_table, k)
+    _ints(past_lens, "past_lens", (batch,), k)
+    cu = cos_p = sin_p = None
     if cu_seqlens is not None:
-        _ints(cu_seqlens, "cu_seqlens", (batch + 1,), k.device)
+        _ints(cu_seqlens, "cu_seqlens", (batch + 1,), k)
+        cu = cu_seqlens.data_ptr()
     elif t != batch:
         raise ValueError(f"{t} tokens for {batch} sequences need cu_seqlens")
     rot = max_pos = 0
@@ -717,25 +752,24 @@ def kv_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, block_table: 
     if cos is not None:
         _check(cos, "cos", torch.float32, 2)
         _check(sin, "sin", torch.float32, 2)
-        if cos.shape != sin.shape or cos.device != k.device or sin.device != k.device:
+        if cos.shape != sin.shape or cos.get_device() != k.get_device() or sin.get_device() != k.get_device():
             raise ValueError(f"cos is {tuple(cos.shape)} on {cos.device}, sin {tuple(sin.shape)} on {sin.device}")
-        max_pos, rot = cos.shape[0], 2 * cos.shape[1]
+        max_pos, rot = cos.shape
+        rot, cos_p, sin_p = 2 * rot, cos.data_ptr(), sin.data_ptr()
     n_heads = 0
     if q is not None:
         if not rot:
             raise ValueError("q is given to be rotated: cos and sin are missing")
         _rows(q, "q", k)
-        if q.shape[0] != t or q.shape[2] != d:
+        tq, n_heads, dq = q.shape
+        if tq != t or dq != d:
             raise ValueError(f"q is {tuple(q.shape)}, k {tuple(k.shape)}")
-        n_heads = q.shape[1]
         q_out = _out_like(q_out, q)
     elif q_out is not None:
         raise ValueError("q_out without q")
-    with torch.cuda.device(k.device):
-        rc = _lib.load().gq_kv_append(cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), n_pages, heads, page,
-                                      d, *_of(k), *_of(v), code, t, block_table.data_ptr(), width, past_lens.data_ptr(), _p(cu_seqlens), batch,
-                                      *_of(q), n_heads, *_of(q_out), _p(cos), _p(sin), max_pos, rot, int(interleaved), _stream(k))
-    _lib.check(rc, "gq_kv_append")
+    _launch("gq_kv_append", k, cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), n_pages, heads, page, d,
+            *_of(k), *_of(v), code, t, block_table.data_ptr(), width, past_lens.data_ptr(), cu, batch, *_of(q), n_heads, *_of(q_out), cos_p, sin_p,
+            max_pos, rot, interleaved)
     return q_out
 
 
@@ -749,28 +783,24 @@ def attention_paged(q: torch.Tensor, cache: PagedCache, block_table: torch.Tenso
     _no_grad(q, out)
     _rows(q, "q")
     code = _dtype_code(q)
-    n_pages, kv_heads, page, d = _check_cache(cache, q.device)
+    n_pages, kv_heads, page, d = _check_cache(cache, q)
     t, heads, dq = q.shape
     if dq != d or kv_heads == 0 or heads % kv_heads:
         raise ValueError(f"q is {tuple(q.shape)}, the cache has {kv_heads} heads of {d}")
-    if not isinstance(block_table, torch.Tensor) or block_table.dim() != 2:
-        raise ValueError("block_table: expected (sequences, pages)")
-    batch, width = block_table.shape
-    _ints(block_table, "block_table", (batch, width), q.device)
-    _ints(seq_lens, "seq_lens", (batch,), q.device)
+    batch, width = _table(block_table, q)
+    _ints(seq_lens, "seq_lens", (batch,), q)
+    cu = None
     if cu_seqlens is not None:
-        _ints(cu_seqlens, "cu_seqlens", (batch + 1,), q.device)
+        _ints(cu_seqlens, "cu_seqlens", (batch + 1,), q)
+        cu = cu_seqlens.data_ptr()
     elif t != batch:
         raise ValueError(f"{t} query tokens for {batch} sequences need cu_seqlens")
     out = _out_like(out, q)
-    lib = _lib.load()
-    with torch.cuda.device(q.device):
-        need = lib.gq_attention_paged_workspace(t, batch, int(cu_seqlens is not None), heads, kv_heads, d, page, width)
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-        rc = lib.gq_attention_paged(*_of(out), *_of(q), code, t, heads, cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
-                                    cache.v_scale.data_ptr(), n_pages, kv_heads, page, d, block_table.data_ptr(), width, seq_lens.data_ptr(),
-                                    _p(cu_seqlens), batch, float(d ** -0.5 if scale is None else scale), _p(ws), need, _stream(q))
-    _lib.check(rc, "gq_attention_paged")
+    need = _lib.load().gq_attention_paged_workspace(t, batch, cu is not None, heads, kv_heads, d, page, width)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    _launch("gq_attention_paged", q, *_of(out), *_of(q), code, t, heads, cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
+            cache.v_scale.data_ptr(), n_pages, kv_heads, page, d, block_table.data_ptr(), width, seq_lens.data_ptr(), cu, batch,
+            d ** -0.5 if scale is None else scale, ws.data_ptr() if need else None, need)
     return out
 
 
@@ -782,23 +812,27 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, ign
     _no_grad(logits)
     if not isinstance(logits, torch.Tensor) or not isinstance(tokens, torch.Tensor):
         raise TypeError("logits and tokens: expected tensors")
-    if logits.device.type != "cuda":
+    if not logits.is_cuda:
         raise ValueError(f"logits: must live on the GPU (got {logits.device}); there is no CPU path")
-    code = 2 if logits.dtype == torch.float32 else _dtype_code(logits)
-    if logits.dim() == 0 or tokens.shape != logits.shape[:-1] or tokens.dtype != torch.int64 or tokens.device != logits.device:
+    code = 2 if logits.dtype is torch.float32 else _dtype_code(logits)
+    shape = tokens.shape
+    if logits.dim() == 0 or shape != logits.shape[:-1] or tokens.dtype is not torch.int64 or tokens.get_device() != logits.get_device():
         raise ValueError(f"logits are {tuple(logits.shape)} on {logits.device}, tokens {tokens.dtype} {tuple(tokens.shape)} on {tokens.device}")
     vocab = logits.shape[-1]
-    rows = logits if logits.dim() == 2 else logits.reshape(-1, vocab) if vocab else logits.reshape(0, 0)
-    if rows.numel() and (rows.stride(1) != 1 and vocab > 1 or rows.stride(0) < vocab):
-        rows = rows.contiguous()
-    n, dev, shape = tokens.numel(), logits.device, tuple(tokens.shape)
-    flat = tokens.reshape(-1).contiguous()
-    lp = torch.empty(shape, dtype=torch.float32, device=dev)
-    ent = torch.empty(shape, dtype=torch.float32, device=dev)
-    tlp = torch.empty(*shape, top, dtype=torch.float32, device=dev) if top > 0 else None
-    tok = torch.empty(*shape, top, dtype=torch.int64, device=dev) if top > 0 else None
-    with torch.cuda.device(dev):
-        rc = _lib.load().gq_token_logprobs(_p(rows), code, n, rows.stride(0) if n else vocab, vocab, _p(flat), int(ignore_index), _p(lp), _p(ent),
-                                           int(top), _p(tlp), _p(tok), _stream(logits))
-    _lib.check(rc, "gq_token_logprobs")
+    if vocab == 0 or not 0 <= top <= vocab:
+        raise ValueError(f"{top} alternatives of {vocab} words")
+    rows = logits if logits.dim() == 2 else logits.reshape(-1, vocab)
+    n = tokens.numel()
+    stride = rows.stride(0) if n > 1 else vocab
+    if n and (vocab > 1 and rows.stride(1) != 1 or stride < vocab):
+        rows, stride = rows.contiguous(), vocab
+    if not tokens.is_contiguous():
+        tokens = tokens.contiguous()
+    lp = torch.empty(shape, dtype=torch.float32, device=logits.device)
+    ent = torch.empty_like(lp)
+    tlp = tok = None
+    if top:
+        tlp, tok = lp.new_empty((*shape, top)), tokens.new_empty((*shape, top))
+    _launch("gq_token_logprobs", logits, rows.data_ptr(), code, n, stride, vocab, tokens.data_ptr(), ignore_index, lp.data_ptr(), ent.data_ptr(), top,
+            tlp.data_ptr() if top else None, tok.data_ptr() if top else None)
     return TokenLogprobs(lp, ent, tlp, tok)
