@@ -16,10 +16,14 @@
 //
 // Bound by HBM: 2 head_dim bytes per cached token and kv head.  A long sequence is cut into runs of tokens for several
 // workgroups, whose (O, M, l) a second kernel joins.
+#include <type_traits>
+
 #include "gq_common.h"
 
 namespace {
 
+constexpr int PA_MAX_SPLITS = 64;   // one wave weighs them
+constexpr int PA_MAX_LEN = 1 << 30;     // longest sequence; tables are narrower (a longer one is NaN)
 constexpr float PA_LOG2E = 1.44269504088896340736f;
 
 struct PagedArgs {
@@ -30,10 +34,13 @@ struct PagedArgs {
     const float *k_scale, *v_scale;
     const int32_t *table, *lens, *cu;       // cu NULL: one query token per sequence
     float *part_o, *part_ml;                // partial results: [token][head][split][head_dim], [token][head][split][2]
-    int64_t n_tokens, n_pages, table_width;
+    int64_t n_tokens;
+    int n_pages, table_width;
     int batch, n_heads, n_kv_heads, group, head_dim, page_log2, tiles_per_split, n_splits, n_items;
     float scale;                            // softmax scale * log2 e
 };
+
+typedef __amdgpu_buffer_rsrc_t pa_rsrc_t;
 
 template <typename T> struct Mfma;
 template <> struct Mfma<_Float16> {
@@ -86,85 +93,146 @@ __device__ __forceinline__ Item find_item(const PagedArgs &a, int item, int mr)
     return {lo, (int)tile, row0, (int)n};
 }
 
-template <int NC>
-struct Tile {
-    u32x4 k[4][NC], v[4 * NC];
-    float ks, vs;
-};
-
-template <typename T, int NC, int NQ>
-__global__ __launch_bounds__(256, NQ == 1 ? 2 : 1) void attention_paged_kernel(const PagedArgs a)
+// ONE: a tile of 64 tokens lies on one page (pages of 64 or 128), whose address is then the same for all lanes: a scalar
+// descriptor and 32-bit lane offsets instead of 64-bit addresses per lane and load.
+template <typename T, int NC, int NQ, bool ONE>
+__global__ __launch_bounds__(256, NQ == 1 ? 3 : (NQ == 2 ? 2 : 1)) void attention_paged_kernel(const PagedArgs a)
 {
     typedef Mfma<T> MM;
     typedef typename MM::vec vec;
     constexpr int MR = 16 * NQ, DP = 64 * NC, DT = 4 * NC;
     constexpr int LROW = DP + 4;   // padded row of the join buffer, in floats
     __shared__ float sm_m[4][MR], sm_l[4][MR];
-    __shared__ __attribute__((aligned(16))) float sm_o[4][16 * LROW];
+    constexpr int QROW = DP + 8;   // padded row of the queries, in elements: 16 rows read side by side spread over the banks
+    union Shared {
+        float o[4][16 * LROW];
+        T q[MR * QROW];
+    };
+    __shared__ __attribute__((aligned(16))) Shared sm;
 
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);   // uniform, so that what follows from it is scalar
     const int head_kv = blockIdx.x % a.n_kv_heads, split = blockIdx.y;
     const Item it = find_item(a, blockIdx.x / a.n_kv_heads, MR);
     if (it.n == 0) return;
     const int d = a.head_dim, page = 1 << a.page_log2;
-    int64_t len = a.lens[it.b];
-    if (len < 0) len = 0;
-    const int64_t n_tiles = (len + 63) >> 6;
-    const int64_t t_lo = (int64_t)split * a.tiles_per_split;
-    const int64_t t_hi = n_tiles < t_lo + a.tiles_per_split ? n_tiles : t_lo + a.tiles_per_split;
+    int len = a.lens[it.b];
+    len = len < 0 ? 0 : (len > PA_MAX_LEN ? PA_MAX_LEN : len);   // (positions and the tile behind them stay below 2^31)
+    const int n_tiles = (len + 63) >> 6;
+    const int t_lo = split * a.tiles_per_split;
+    const int t_hi = n_tiles < t_lo + a.tiles_per_split ? n_tiles : t_lo + a.tiles_per_split;
     if (split > 0 && t_lo >= n_tiles) return;
 
-    // this lane's query rows (column m of each 16-row tile) and the last position each may see
-    vec qf[NQ][2 * NC];
-    int64_t last[NQ];
+    // the query rows go to LDS (registers are what the loads in flight need), 0 where there is no row or channel
+    for (int i = threadIdx.x; i < MR * DP / 8; i += 256) {
+        const int rr = i / (DP / 8), ch = 8 * (i - rr * (DP / 8)), r = it.tile * MR + rr, tok = r / a.group;
+        u32x4 raw = {0, 0, 0, 0};
+        if (tok < it.n && ch < d)
+            raw = *reinterpret_cast<const u32x4 *>((const T *)a.q + (it.row0 + tok) * a.q_tok + (int64_t)(head_kv * a.group + (r - tok * a.group)) * a.q_head + ch);
+        *reinterpret_cast<u32x4 *>(&sm.q[rr * QROW + ch]) = raw;
+    }
+    // the last position that this lane's row (column m of each 16-row tile) sees
+    int last[NQ];
 #pragma unroll
     for (int nt = 0; nt < NQ; ++nt) {
-        const int r = it.tile * MR + 16 * nt + m, tok = r / a.group;
-        const bool live = tok < it.n;
-        last[nt] = live ? len - it.n + tok : -1;
-        const T *qp = (const T *)a.q + (it.row0 + (live ? tok : 0)) * a.q_tok + (int64_t)(head_kv * a.group + (r - tok * a.group)) * a.q_head;
-#pragma unroll
-        for (int s = 0; s < 2 * NC; ++s) {
-            const int ch = 64 * (s >> 1) + 16 * g + 8 * (s & 1);
-            u32x4 raw = {0, 0, 0, 0};
-            if (live && ch < d) raw = *reinterpret_cast<const u32x4 *>(qp + ch);
-            __builtin_memcpy(&qf[nt][s], &raw, 16);
-        }
+        const int tok = (it.tile * MR + 16 * nt + m) / a.group;
+        last[nt] = tok < it.n ? len - it.n + tok : -1;
     }
+    __syncthreads();
 
+    // The pages of a tile of 64 tokens from this lane's two points of view: of the keys of tokens 16 (m / 4).. and of
+    // the values of tokens 16 g.. (ONE: the same for all, in scalar registers).  The entries of the table are fetched a
+    // tile before they are used, and in front of that tile's loads: waits are for loads in the order they were issued.
     bool bad = false;   // a token that should be there lies on no page
     const int32_t *table = a.table + (int64_t)it.b * a.table_width;
-    const int64_t head_bytes = (int64_t)page * d;
-    const auto page_of = [&](int64_t tok) -> int64_t {   // -1: behind the sequence, or no page
-        if (tok >= len) return -1;
-        const int64_t i = tok >> a.page_log2;
-        const int64_t id = i < a.table_width ? (int64_t)table[i] : -1;
-        if (id < 0 || id >= a.n_pages) {
-            bad = true;
-            return -1;
-        }
-        return id;
+    struct Pages {
+        int k, v;
     };
-    const auto load = [&](int64_t t, Tile<NC> &w) {
-        const int64_t tk = t * 64 + 16 * (m >> 2), tv = t * 64 + 16 * g;
-        const int64_t pk = page_of(tk), pv = page_of(tv);
-        const int64_t bk = pk * a.n_kv_heads + head_kv, bv = pv * a.n_kv_heads + head_kv;
-        const uint8_t *kp = a.k_codes + bk * head_bytes + ((tk & (page - 1)) + (m & 3)) * d + 16 * g;
-        const uint8_t *vp = a.v_codes + bv * head_bytes + (int64_t)m * page + (tv & (page - 1));
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                w.k[i][c] = u32x4{0, 0, 0, 0};
-                if (pk >= 0 && 64 * c + 16 * g < d) w.k[i][c] = *reinterpret_cast<const u32x4 *>(kp + 4 * i * d + 64 * c);
-            }
-#pragma unroll
-        for (int t2 = 0; t2 < DT; ++t2) {
-            w.v[t2] = u32x4{0, 0, 0, 0};
-            if (pv >= 0 && 16 * t2 < d) w.v[t2] = *reinterpret_cast<const u32x4 *>(vp + 16 * t2 * page);
+    const auto entry = [&](int tok) {
+        const int i = tok >> a.page_log2;
+        return tok < len && i < a.table_width ? table[i] : -1;
+    };
+    const auto fetch_pages = [&](int t) -> Pages {
+        if constexpr (ONE) {
+            const int id = entry(t * 64);
+            return {id, id};
+        } else {
+            return {entry(t * 64 + 16 * (m >> 2)), entry(t * 64 + 16 * g)};
         }
-        w.ks = pv >= 0 ? a.k_scale[bv] : 1.f;
-        w.vs = pv >= 0 ? a.v_scale[bv] : 1.f;
+    };
+    // page 0 stands in for no page
+    const auto check_pages = [&](Pages p, int t) -> Pages {
+        const auto one = [&](int id, int tok) {
+            if (id >= 0 && id < a.n_pages) return id;
+            bad |= tok < len;
+            return 0;
+        };
+        if constexpr (ONE) {
+            const int id = one(p.k, t * 64);
+            return {id, id};
+        } else {
+            return {one(p.k, t * 64 + 16 * (m >> 2)), one(p.v, t * 64 + 16 * g)};
+        }
+    };
+    // What lies behind the sequence, on no page or behind head_dim is read from a place that exists (page 0, the row's
+    // first channels, the first channels' rows) and does not count: such scores are masked or met by zeros of q, such
+    // values are cleared or their results not written.
+    const int head_bytes = page * d;
+    // The lane's offsets are worked out anew for each tile (from a lane number the compiler does not see through): kept
+    // over the loop they are the first thing it spills, and a reload waits for every load in flight.
+    const auto lane_again = [&]() {
+        int x = lane;
+        asm volatile("" : "+v"(x));
+        return x;
+    };
+    const auto k_offset = [&](int l, int c) {
+        const int mm = l & 15, gg = l >> 4;
+        return (unsigned)((mm & 3) * d + (ONE ? 16 * (mm >> 2) * d : 0) + (64 * c + 16 * gg < d ? 64 * c + 16 * gg : 0));
+    };
+    u32x4 kr[4][NC], vr[DT];
+    float ks, vs, ks_next, vs_next;
+    // ONE: a buffer descriptor of the page's block (scalar), 32-bit lane offsets
+    const auto block_of = [&](const uint8_t *codes, int id) {
+        return __builtin_amdgcn_make_buffer_rsrc((void *)(codes + ((int64_t)id * a.n_kv_heads + head_kv) * head_bytes), 0, head_bytes, 0x00020000);
+    };
+    const auto load_k = [&](int t, int id) {
+        const int l = lane_again();
+        unsigned k_off[NC];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) k_off[c] = k_offset(l, c);
+        if constexpr (ONE) {
+            const pa_rsrc_t rs = block_of(a.k_codes, id);
+            const int at = ((t * 64) & (page - 1)) * d;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int c = 0; c < NC; ++c) kr[i][c] = __builtin_amdgcn_raw_buffer_load_b128(rs, (int)k_off[c], at + 4 * i * d, 0);
+        } else {
+            const uint8_t *p = a.k_codes + ((int64_t)id * a.n_kv_heads + head_kv) * head_bytes + ((t * 64 + 16 * (m >> 2)) & (page - 1)) * d;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int c = 0; c < NC; ++c) kr[i][c] = *reinterpret_cast<const u32x4 *>(p + 4 * i * d + k_off[c]);
+        }
+    };
+    const auto load_v = [&](int t, int id) {
+        const int l = lane_again();
+        const unsigned v_off = (l & 15) * page + (ONE ? 16 * (l >> 4) : 0);
+        if constexpr (ONE) {
+            const pa_rsrc_t rs = block_of(a.v_codes, id);
+            const int at = (t * 64) & (page - 1);
+#pragma unroll
+            for (int t2 = 0; t2 < DT; ++t2) vr[t2] = __builtin_amdgcn_raw_buffer_load_b128(rs, (int)v_off, at + (16 * t2 < d ? 16 * t2 * page : 0), 0);
+        } else {
+            const uint8_t *p = a.v_codes + ((int64_t)id * a.n_kv_heads + head_kv) * head_bytes + ((t * 64 + 16 * g) & (page - 1));
+#pragma unroll
+            for (int t2 = 0; t2 < DT; ++t2) vr[t2] = *reinterpret_cast<const u32x4 *>(p + (16 * t2 < d ? 16 * t2 * page : 0) + v_off);
+        }
+    };
+    const auto load_scales = [&](int id) {
+        const int64_t block = (int64_t)id * a.n_kv_heads + head_kv;
+        ks_next = a.k_scale[block];
+        vs_next = a.v_scale[block];
     };
 
     f32x4 o[NQ][DT];
@@ -177,30 +245,52 @@ __global__ __launch_bounds__(256, NQ == 1 ? 2 : 1) void attention_paged_kernel(c
         for (int t2 = 0; t2 < DT; ++t2) o[nt][t2] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     // tokens from here on are hidden from some row: behind the sequence, or after a query token of it
-    const int64_t partly = len - it.n + 1;
+    const int partly = len - it.n + 1;
 
-    Tile<NC> cur, nxt;
-    int64_t t = t_lo + wave;
-    if (t < t_hi) load(t, cur);
-    for (; t < t_hi; t += 4) {
-        if (t + 4 < t_hi) load(t + 4, nxt);
+    // One set of registers: the next tile's keys are loaded as soon as this one's have met the queries, its values after
+    // this one's have met the weights.
+    int t = t_lo + wave;
+    Pages next = {0, 0};
+    if (t < t_hi) {
+        const Pages first = check_pages(fetch_pages(t), t);
+        if (t + 4 < t_hi) next = fetch_pages(t + 4);
+        load_k(t, first.k);
+        load_v(t, first.v);
+        load_scales(first.v);
+    }
+    const auto step = [&](auto masked) {
+        const bool more = t + 4 < t_hi;
+        ks = ks_next;
+        vs = vs_next;
+        Pages now = next;
+        if (t + 8 < t_hi) next = fetch_pages(t + 8);
         f32x4 s[NQ][4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int nt = 0; nt < NQ; ++nt)
 #pragma unroll
-            for (int nt = 0; nt < NQ; ++nt) s[nt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int i = 0; i < 4; ++i) s[nt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int c = 0; c < NC; ++c)
+        for (int c = 0; c < NC; ++c)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const vec kf = MM::decode(cur.k[i][c][2 * h], cur.k[i][c][2 * h + 1]);
+            for (int h = 0; h < 2; ++h) {
+                vec qf[NQ];
 #pragma unroll
-                    for (int nt = 0; nt < NQ; ++nt) s[nt][i] = MM::run(kf, qf[nt][2 * c + h], s[nt][i]);
+                for (int nt = 0; nt < NQ; ++nt) qf[nt] = *reinterpret_cast<const vec *>(&sm.q[(16 * nt + m) * QROW + 64 * c + 16 * g + 8 * h]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const vec kf = MM::decode(kr[i][c][2 * h], kr[i][c][2 * h + 1]);
+#pragma unroll
+                    for (int nt = 0; nt < NQ; ++nt) s[nt][i] = MM::run(kf, qf[nt], s[nt][i]);
                 }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        if (more) {
+            now = check_pages(now, t + 4);
+            load_k(t + 4, now.k);
+            load_scales(now.v);
         }
-        const float vs = fmaxf(cur.vs, 1e-30f);   // a scale of 0 must not become an infinite weight
-        const float mul = a.scale * cur.ks, add = __builtin_amdgcn_logf(vs), inv = 1.f / vs;
-        const bool masked = (t + 1) * 64 > partly;
+        vs = fmaxf(vs, 1e-30f);   // a scale of 0 must not become an infinite weight
+        const float mul = a.scale * ks, add = __builtin_amdgcn_logf(vs), inv = 1.f / vs;
         f16x8 p[NQ][2];
 #pragma unroll
         for (int nt = 0; nt < NQ; ++nt) {
@@ -240,16 +330,16 @@ __global__ __launch_bounds__(256, NQ == 1 ? 2 : 1) void attention_paged_kernel(c
         }
         bool apart = false;   // a NaN among the values of a tile that is not visible to every row
         if (masked) {
-            const int64_t left = len - (t * 64 + 16 * g);   // of this lane's 16 tokens
+            const int left = len - (t * 64 + 16 * g);   // of this lane's 16 tokens
             bool nan = false;
 #pragma unroll
             for (int t2 = 0; t2 < DT; ++t2)
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
-                    const int64_t k = left - 4 * w;
+                    const int k = left - 4 * w;
                     const unsigned keep = k >= 4 ? 0xffffffffu : (k <= 0 ? 0u : (1u << (8 * k)) - 1);
-                    const unsigned x = cur.v[t2][w] & keep;
-                    cur.v[t2][w] = x;
+                    const unsigned x = vr[t2][w] & keep;
+                    vr[t2][w] = x;
                     // a byte is NaN where its low seven bits are all set: then adding 1 carries into the eighth
                     nan |= (((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
                 }
@@ -257,13 +347,15 @@ __global__ __launch_bounds__(256, NQ == 1 ? 2 : 1) void attention_paged_kernel(c
         }
         if (!apart) {
 #pragma unroll
-            for (int t2 = 0; t2 < DT; ++t2)
+            for (int t2 = 0; t2 < DT; ++t2) {
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    const f16x8 vf = Mfma<_Float16>::decode(cur.v[t2][2 * u], cur.v[t2][2 * u + 1]);
+                    const f16x8 vf = Mfma<_Float16>::decode(vr[t2][2 * u], vr[t2][2 * u + 1]);
 #pragma unroll
                     for (int nt = 0; nt < NQ; ++nt) o[nt][t2] = Mfma<_Float16>::run(vf, p[nt][u], o[nt][t2]);
                 }
+                __builtin_amdgcn_sched_barrier(0);
+            }
         } else {
             // 0 * NaN is NaN: one token at a time, added only to the rows that see it
             for (int tok = 0; tok < 64; ++tok) {
@@ -273,7 +365,7 @@ __global__ __launch_bounds__(256, NQ == 1 ? 2 : 1) void attention_paged_kernel(c
                     unsigned w[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        w[i] = (tok >> 4) == g && ((tok >> 2) & 3) == i ? cur.v[t2][i] & (0xffu << (8 * (tok & 3))) : 0u;
+                        w[i] = (tok >> 4) == g && ((tok >> 2) & 3) == i ? vr[t2][i] & (0xffu << (8 * (tok & 3))) : 0u;
 #pragma unroll
                     for (int nt = 0; nt < NQ; ++nt) {
                         f32x4 x = Mfma<_Float16>::run(Mfma<_Float16>::decode(w[0], w[1]), p[nt][0], f32x4{0.f, 0.f, 0.f, 0.f});
@@ -283,8 +375,11 @@ __global__ __launch_bounds__(256, NQ == 1 ? 2 : 1) void attention_paged_kernel(c
                 }
             }
         }
-        cur = nxt;
-    }
+        if (more) load_v(t + 4, now.v);
+    };
+    // (kept in order: left to itself the scheduler decodes a whole tile ahead and spills)
+    for (; t < t_hi && (t + 1) * 64 <= partly; t += 4) step(std::false_type());
+    for (; t < t_hi; t += 4) step(std::true_type());
 
     // join the four waves
     const bool any_bad = __any(bad);
@@ -304,13 +399,13 @@ __global__ __launch_bounds__(256, NQ == 1 ? 2 : 1) void attention_paged_kernel(c
         const int rm = 16 * nt + m;
         const float all = fmaxf(fmaxf(sm_m[0][rm], sm_m[1][rm]), fmaxf(sm_m[2][rm], sm_m[3][rm]));
         const float f = mx[nt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx[nt] - all);
-        if (nt > 0) __syncthreads();
+        if (nt > 0) __syncthreads();   // (before the first, all waves are done with the queries)
 #pragma unroll
         for (int t2 = 0; t2 < DT; ++t2) {
             f32x4 x = o[nt][t2];
 #pragma unroll
             for (int j = 0; j < 4; ++j) x[j] *= f;
-            *reinterpret_cast<f32x4 *>(&sm_o[wave][m * LROW + 16 * t2 + 4 * g]) = x;
+            *reinterpret_cast<f32x4 *>(&sm.o[wave][m * LROW + 16 * t2 + 4 * g]) = x;
         }
         __syncthreads();
         const int row = threadIdx.x >> 4, rr = 16 * nt + row, r = it.tile * MR + rr, tok = r / a.group;
@@ -322,7 +417,7 @@ __global__ __launch_bounds__(256, NQ == 1 ? 2 : 1) void attention_paged_kernel(c
         const int64_t qrow = it.row0 + tok;
         for (int ch = 4 * (threadIdx.x & 15); ch < d; ch += 64) {
             f32x4 x = {0.f, 0.f, 0.f, 0.f};
-            for (int w = 0; w < 4; ++w) x += *reinterpret_cast<const f32x4 *>(&sm_o[w][row * LROW + ch]);
+            for (int w = 0; w < 4; ++w) x += *reinterpret_cast<const f32x4 *>(&sm.o[w][row * LROW + ch]);
             if (a.n_splits > 1) {
                 *reinterpret_cast<f32x4 *>(a.part_o + ((qrow * a.n_heads + head) * a.n_splits + split) * d + ch) = x;
             } else {
@@ -342,15 +437,15 @@ __global__ __launch_bounds__(256, NQ == 1 ? 2 : 1) void attention_paged_kernel(c
     }
 }
 
-// Joins a row's partial results: O = sum_s 2^(M_s - M) O_s / sum_s 2^(M_s - M) l_s.  One wave per row.
+// Joins a row's partial results: O = sum_s 2^(M_s - M) O_s / sum_s 2^(M_s - M) l_s.  One workgroup per row: 8 groups of
+// 32 lanes take every eighth run (4 channels a lane), so that a row of many runs is few loads deep.
 template <typename T>
 __global__ __launch_bounds__(256) void attention_paged_join_kernel(const PagedArgs a)
 {
-    const int lane = threadIdx.x & 63;
-    const int64_t idx = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (idx >= a.n_tokens * a.n_heads) return;
-    const int64_t tok = idx / a.n_heads;
-    const int head = (int)(idx - tok * a.n_heads);
+    __shared__ float sm_f[PA_MAX_SPLITS], sm_sum;
+    __shared__ f32x4 sm_x[8][32];
+    const int64_t idx = blockIdx.x, tok = idx / a.n_heads;
+    const int head = (int)(idx - tok * a.n_heads), tid = threadIdx.x, part = tid >> 5, ch = 4 * (tid & 31);
     int b = (int)tok;
     if (a.cu) {
         if (tok < a.cu[0] || tok >= a.cu[a.batch]) return;   // behind the last sequence: left as it is
@@ -363,30 +458,40 @@ __global__ __launch_bounds__(256) void attention_paged_join_kernel(const PagedAr
         b = lo;
         if (a.cu[b + 1] <= tok || a.cu[b] < 0 || a.cu[b + 1] > a.n_tokens) return;   // not rising: the first kernel left it out
     }
-    const int64_t len = a.lens[b] < 0 ? 0 : a.lens[b], n_tiles = (len + 63) >> 6;
-    const int64_t used64 = (n_tiles + a.tiles_per_split - 1) / a.tiles_per_split;
-    const int used = used64 < 1 ? 1 : (used64 > a.n_splits ? a.n_splits : (int)used64);
-    const float *ml = a.part_ml + idx * a.n_splits * 2;
-    const float *po = a.part_o + idx * a.n_splits * a.head_dim;
-    float top = -INFINITY;
-    for (int s = lane; s < used; s += 64) top = fmaxf(top, ml[2 * s]);
+    const int len = a.lens[b] < 0 ? 0 : (a.lens[b] > PA_MAX_LEN ? PA_MAX_LEN : a.lens[b]);
+    const int wanted = ((len + 63) / 64 + a.tiles_per_split - 1) / a.tiles_per_split;
+    const int used = wanted < 1 ? 1 : (wanted > a.n_splits ? a.n_splits : wanted);
+    if (tid < 64) {   // PA_MAX_SPLITS runs at most: one wave weighs them
+        const float *ml = a.part_ml + (idx * a.n_splits + tid) * 2;
+        const float mx = tid < used ? ml[0] : -INFINITY, l = tid < used ? ml[1] : 0.f;
+        float top = mx;
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
-    const float ref = top == -INFINITY ? 0.f : top;
-    float sum = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
-    const int ch = 4 * lane;
-    for (int s = 0; s < used; ++s) {
-        const float f = __builtin_amdgcn_exp2f(ml[2 * s] - ref);
-        sum += ml[2 * s + 1] * (ml[2 * s] == -INFINITY && ml[2 * s + 1] != 0.f ? 1.f : f);
-        if (ch < a.head_dim) {
-            const f32x4 v = *reinterpret_cast<const f32x4 *>(po + (int64_t)s * a.head_dim + ch);
+        for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+        const float f = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - top);
+        float sum = mx == -INFINITY ? l : l * f;   // (0 without a key, NaN for a bad table)
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
+        sm_f[tid] = f;
+        // more tokens than the table has pages for
+        if (tid == 0) sm_sum = wanted > a.n_splits ? NAN : sum;
+    }
+    __syncthreads();
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+    if (ch < a.head_dim)
+        for (int s = part; s < used; s += 8) {
+            const f32x4 v = *reinterpret_cast<const f32x4 *>(a.part_o + (idx * a.n_splits + s) * a.head_dim + ch);
+            const float f = sm_f[s];
+#pragma unroll
             for (int j = 0; j < 4; ++j) x[j] = fmaf(v[j], f, x[j]);
         }
-    }
-    // fewer splits than the sequence has tokens for: the table is too narrow for its length
-    if (used64 > a.n_splits) sum = NAN;
-    if (ch < a.head_dim) {
+    sm_x[part][tid & 31] = x;
+    __syncthreads();
+    if (part == 0 && ch < a.head_dim) {
+#pragma unroll
+        for (int p = 1; p < 8; ++p) x += sm_x[p][tid];
+        const float sum = sm_sum;
         T y[4];
+#pragma unroll
         for (int j = 0; j < 4; ++j) y[j] = (T)(sum == 0.f ? 0.f : x[j] / sum);
         u32x2 raw;
         __builtin_memcpy(&raw, y, 8);
@@ -412,7 +517,7 @@ Plan paged_plan(int64_t n_tokens, int64_t batch, bool ragged, int n_heads, int n
     const int64_t tiles = gq_cdiv(table_width * page, 64), wgs = p.n_items * n_kv_heads;
     int64_t splits = gq_cdiv(2048, wgs);
     splits = std::min<int64_t>(splits, gq_cdiv(tiles, 4));
-    splits = std::max<int64_t>(1, std::min<int64_t>(splits, 64));
+    splits = std::max<int64_t>(1, std::min<int64_t>(splits, PA_MAX_SPLITS));
     p.tiles_per_split = (int)std::max<int64_t>(4, gq_round_up(gq_cdiv(tiles, splits), 4));
     p.n_splits = (int)std::max<int64_t>(1, gq_cdiv(tiles, p.tiles_per_split));
     return p;
@@ -422,14 +527,18 @@ bool paged_sizes_ok(int64_t n_tokens, int64_t batch, int n_heads, int n_kv_heads
 {
     return n_tokens >= 0 && n_tokens < ((int64_t)1 << 31) && batch >= 0 && batch < (1 << 24) && n_kv_heads > 0 && n_heads > 0 && n_heads <= 65536 &&
            n_heads % n_kv_heads == 0 && head_dim >= 16 && head_dim <= 128 && head_dim % 16 == 0 &&
-           (page == 16 || page == 32 || page == 64 || page == 128) && table_width >= 0 && table_width < ((int64_t)1 << 24);
+           (page == 16 || page == 32 || page == 64 || page == 128) && table_width >= 0 && table_width * page < PA_MAX_LEN;
 }
 
 template <typename T>
 int launch_paged(const PagedArgs &a, const Plan &p, hipStream_t s)
 {
     const dim3 grid((unsigned)(p.n_items * a.n_kv_heads), (unsigned)p.n_splits);
-#define GQ_PA(NC, NQ) hipLaunchKernelGGL((attention_paged_kernel<T, NC, NQ>), grid, dim3(256), 0, s, a)
+#define GQ_PA(NC, NQ)                                                                                                   \
+    do {                                                                                                                \
+        if (a.page_log2 >= 6) hipLaunchKernelGGL((attention_paged_kernel<T, NC, NQ, true>), grid, dim3(256), 0, s, a);  \
+        else hipLaunchKernelGGL((attention_paged_kernel<T, NC, NQ, false>), grid, dim3(256), 0, s, a);                  \
+    } while (0)
     if (a.head_dim <= 64) {
         if (p.nq == 1) GQ_PA(1, 1);
         else if (p.nq == 2) GQ_PA(1, 2);
@@ -442,7 +551,7 @@ int launch_paged(const PagedArgs &a, const Plan &p, hipStream_t s)
 #undef GQ_PA
     GQ_LAUNCH_CHECK();
     if (p.n_splits > 1) {
-        hipLaunchKernelGGL(attention_paged_join_kernel<T>, dim3((unsigned)gq_cdiv(a.n_tokens * a.n_heads, 4)), dim3(256), 0, s, a);
+        hipLaunchKernelGGL(attention_paged_join_kernel<T>, dim3((unsigned)(a.n_tokens * a.n_heads)), dim3(256), 0, s, a);
         GQ_LAUNCH_CHECK();
     }
     return GQ_OK;
@@ -472,14 +581,15 @@ extern "C" int gq_attention_paged(void *out, int64_t out_token_stride, int64_t o
                (long long)batch);
     GQ_REQUIRE(softmax_scale > 0.f && softmax_scale < INFINITY, "gq_attention_paged: the softmax scale must be positive and finite");
     if (n_tokens == 0 || batch == 0) return GQ_OK;
-    GQ_REQUIRE(out && q && seq_lens && (table_width == 0 || block_table) && (n_pages == 0 || (k_codes && v_codes && k_scale && v_scale)),
+    GQ_REQUIRE(out && q && seq_lens && (table_width == 0 || block_table) && k_codes && v_codes && k_scale && v_scale,
                "gq_attention_paged: NULL pointer");
     GQ_REQUIRE(q_token_stride % 8 == 0 && q_head_stride % 8 == 0 && out_token_stride % 8 == 0 && out_head_stride % 8 == 0,
                "gq_attention_paged: strides must be multiples of 8 elements");
     GQ_REQUIRE((((uintptr_t)out | (uintptr_t)q | (uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)workspace) & 15) == 0,
                "gq_attention_paged: pointers must be 16-byte aligned");
     const Plan p = paged_plan(n_tokens, batch, cu_seqlens != nullptr, n_heads, n_kv_heads, page, table_width);
-    GQ_REQUIRE(p.n_items * n_kv_heads < ((int64_t)1 << 31), "gq_attention_paged: too many query rows for one call");
+    GQ_REQUIRE(n_pages > 0, "gq_attention_paged: a cache without pages");
+    GQ_REQUIRE(n_pages < ((int64_t)1 << 31) && p.n_items * n_kv_heads < ((int64_t)1 << 31) && n_tokens * n_heads < ((int64_t)1 << 31), "gq_attention_paged: too many query rows for one call");
     const size_t need = p.n_splits == 1 ? 0 : (size_t)n_tokens * n_heads * p.n_splits * (head_dim + 4) * sizeof(float);
     if (workspace_bytes < need || (need && !workspace)) {
         gq_set_error("gq_attention_paged: workspace of %zu bytes, %zu needed", workspace_bytes, need);
@@ -491,7 +601,7 @@ extern "C" int gq_attention_paged(void *out, int64_t out_token_stride, int64_t o
     a.table = block_table, a.lens = seq_lens, a.cu = cu_seqlens;
     a.part_o = (float *)workspace;
     a.part_ml = (float *)workspace + (size_t)n_tokens * n_heads * p.n_splits * head_dim;
-    a.n_tokens = n_tokens, a.n_pages = n_pages, a.table_width = table_width;
+    a.n_tokens = n_tokens, a.n_pages = (int)n_pages, a.table_width = (int)table_width;
     a.batch = (int)batch, a.n_heads = n_heads, a.n_kv_heads = n_kv_heads, a.group = n_heads / n_kv_heads, a.head_dim = head_dim;
     a.page_log2 = __builtin_ctz((unsigned)page), a.tiles_per_split = p.tiles_per_split, a.n_splits = p.n_splits, a.n_items = (int)p.n_items;
     a.scale = softmax_scale * PA_LOG2E;

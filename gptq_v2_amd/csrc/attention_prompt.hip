@@ -61,7 +61,8 @@ __global__ __launch_bounds__(256, 2) void attention_prompt_kernel(const PromptAr
     constexpr int STEPS = DP / 16, DT = DP / 32;
     __shared__ __attribute__((aligned(1024))) T sm_k[2][AP_K * DP], sm_v[2][AP_K * DP];
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, h = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);   // uniform, so that what follows from it is scalar
     // workgroups of one head group run on one XCD (consecutive blocks go round the 8) and share its L2; long tiles first
     int head, item;
     if ((a.n_heads & 7) == 0) {
