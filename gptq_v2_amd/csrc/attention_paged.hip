@@ -6,10 +6,15 @@
 // The value's scale sits in the exponent, so the weights that meet the codes on the matrix core are at most 1 whatever
 // the scales are, and the denominator takes it out again in 32 bits.
 //
-// A wave takes 64 tokens at a time, all from registers: S^T = K Q^T (16 x 16 x 32 tiles: tokens by query rows) and
-// O^T = V^T P^T.  Row 4 g + i of the S^T tile a stands for token 16 g + 4 a + i; lane group g then holds, as the tiles'
-// results, the weights of the 16 adjacent tokens 16 g .. 16 g + 15 of its query row -- exactly what it has to supply as
-// the operand P^T, and exactly the 16 bytes it loads of a row of V^T.  No value crosses lanes but for the maximum.
+// A wave takes 64 tokens at a time: S^T = K Q^T (16 x 16 x 32 tiles: tokens by query rows) and O^T = V^T P^T.  Row
+// 4 g + i of the S^T tile a stands for token 16 g + 4 a + i; lane group g then holds, as the tiles' results, the weights of
+// the 16 adjacent tokens 16 g .. 16 g + 15 of its query row -- exactly what it has to supply as the operand P^T, next to
+// the 16 bytes of a row of V^T.  No value crosses lanes but for the maximum.
+// The codes come through LDS: the matrix operands want 16 lanes in 16 different rows, and loads of 16 bytes each from 16
+// rows reach 4.7 TB/s where the same bytes in order reach 6.  The asynchronous copy brings whole lines, its 16-byte
+// pieces permuted within 128 so that the operand reads touch all banks.  A wave has its own buffers and waits for
+// nobody: the next tile's keys are under way as soon as this one's have met the queries, its values after this one's
+// have met the weights.
 // The rows are the query heads that share a kv head (times the tokens of the sequence); the cache is read once for
 // every 16 NQ of them.  e4m3 codes are exact in either 16-bit type: Q K^T runs in q's type, P V in fp16 (w <= 1 keeps
 // 11 bits there, against 8 in bf16).
@@ -40,7 +45,32 @@ struct PagedArgs {
     float scale;                            // softmax scale * log2 e
 };
 
-typedef __amdgpu_buffer_rsrc_t pa_rsrc_t;
+// A uniform load of what no kernel writes meanwhile, by the scalar unit: it is not counted with the copies, whose
+// order the waits below rely on.
+template <typename V>
+__device__ __forceinline__ V pa_scalar_load(const V *p, int64_t i)
+{
+    return *(const V __attribute__((address_space(4))) *)(uintptr_t)(p + i);
+}
+
+// At most N of the wave's copies are left under way; the oldest end first.
+template <int N>
+__device__ __forceinline__ void pa_wait()
+{
+    static_assert(N == 0 || N == 4 || N == 8, "");
+    if constexpr (N == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+    else if constexpr (N == 4) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// The wave's reads of a buffer have returned: a copy may overwrite it.
+__device__ __forceinline__ void pa_reads_done()
+{
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
 
 template <typename T> struct Mfma;
 template <> struct Mfma<_Float16> {
@@ -93,22 +123,24 @@ __device__ __forceinline__ Item find_item(const PagedArgs &a, int item, int mr)
     return {lo, (int)tile, row0, (int)n};
 }
 
-// ONE: a tile of 64 tokens lies on one page (pages of 64 or 128), whose address is then the same for all lanes: a scalar
-// descriptor and 32-bit lane offsets instead of 64-bit addresses per lane and load.
-template <typename T, int NC, int NQ, bool ONE>
-__global__ __launch_bounds__(256, NQ == 1 ? 3 : (NQ == 2 ? 2 : 1)) void attention_paged_kernel(const PagedArgs a)
+// The place of piece p (of 16 bytes) of the 128 bytes R of a buffer: pieces that are read together lie in different banks.
+// Values are read 8 rows in order; keys in two runs of 4 rows, 16 apart.
+template <int DP>
+__device__ __forceinline__ int pa_key_swizzle(int R) { return DP == 128 ? (R & 3) | ((R >> 2) & 4) : (R & 1) | ((R >> 2) & 2); }
+
+// SUB: 16-token groups of a tile on one page (pages of 16, 32 and 64 or more: 1, 2, 4)
+template <typename T, int NC, int NQ, int SUB>
+__global__ __launch_bounds__(256, NQ == 4 ? 1 : 2) void attention_paged_kernel(const PagedArgs a)
 {
     typedef Mfma<T> MM;
     typedef typename MM::vec vec;
     constexpr int MR = 16 * NQ, DP = 64 * NC, DT = 4 * NC;
-    constexpr int LROW = DP + 4;   // padded row of the join buffer, in floats
     __shared__ float sm_m[4][MR], sm_l[4][MR];
     constexpr int QROW = DP + 8;   // padded row of the queries, in elements: 16 rows read side by side spread over the banks
-    union Shared {
-        float o[4][16 * LROW];
-        T q[MR * QROW];
-    };
-    __shared__ __attribute__((aligned(16))) Shared sm;
+    constexpr int NP = 4 / SUB, COPIES = DP / 16;  // pages of a tile; copy instructions (1 KB each) of its keys, of its values
+    // Per wave: keys by token, values by channel.  Two objects, so that the compiler's own waits tell their copies apart.
+    __shared__ __attribute__((aligned(1024))) uint8_t sm_k[4][64 * DP], sm_v[4][64 * DP];
+    __shared__ __attribute__((aligned(16))) T sm_q[MR * QROW];
 
     const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);   // uniform, so that what follows from it is scalar
@@ -129,7 +161,7 @@ __global__ __launch_bounds__(256, NQ == 1 ? 3 : (NQ == 2 ? 2 : 1)) void attentio
         u32x4 raw = {0, 0, 0, 0};
         if (tok < it.n && ch < d)
             raw = *reinterpret_cast<const u32x4 *>((const T *)a.q + (it.row0 + tok) * a.q_tok + (int64_t)(head_kv * a.group + (r - tok * a.group)) * a.q_head + ch);
-        *reinterpret_cast<u32x4 *>(&sm.q[rr * QROW + ch]) = raw;
+        *reinterpret_cast<u32x4 *>(&sm_q[rr * QROW + ch]) = raw;
     }
     // the last position that this lane's row (column m of each 16-row tile) sees
     int last[NQ];
@@ -140,99 +172,74 @@ __global__ __launch_bounds__(256, NQ == 1 ? 3 : (NQ == 2 ? 2 : 1)) void attentio
     }
     __syncthreads();
 
-    // The pages of a tile of 64 tokens from this lane's two points of view: of the keys of tokens 16 (m / 4).. and of
-    // the values of tokens 16 g.. (ONE: the same for all, in scalar registers).  The entries of the table are fetched a
-    // tile before they are used, and in front of that tile's loads: waits are for loads in the order they were issued.
+    // The pages of a tile, in scalar registers; the entries of the table are fetched a tile before they are used.
     bool bad = false;   // a token that should be there lies on no page
     const int32_t *table = a.table + (int64_t)it.b * a.table_width;
     struct Pages {
-        int k, v;
+        int id[NP];
     };
-    const auto entry = [&](int tok) {
-        const int i = tok >> a.page_log2;
-        return tok < len && i < a.table_width ? table[i] : -1;
-    };
-    const auto fetch_pages = [&](int t) -> Pages {
-        if constexpr (ONE) {
-            const int id = entry(t * 64);
-            return {id, id};
-        } else {
-            return {entry(t * 64 + 16 * (m >> 2)), entry(t * 64 + 16 * g)};
+    const auto fetch_pages = [&](int t) {
+        Pages p;
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            const int tok = t * 64 + 16 * SUB * i, e = tok >> a.page_log2;
+            p.id[i] = tok < len && e < a.table_width ? pa_scalar_load(table, e) : -1;
         }
+        return p;
     };
-    // page 0 stands in for no page
-    const auto check_pages = [&](Pages p, int t) -> Pages {
-        const auto one = [&](int id, int tok) {
-            if (id >= 0 && id < a.n_pages) return id;
-            bad |= tok < len;
-            return 0;
-        };
-        if constexpr (ONE) {
-            const int id = one(p.k, t * 64);
-            return {id, id};
-        } else {
-            return {one(p.k, t * 64 + 16 * (m >> 2)), one(p.v, t * 64 + 16 * g)};
-        }
+    // page 0 stands in for no page: what is read there is masked, or the row is NaN
+    const auto check_pages = [&](Pages p, int t) {
+#pragma unroll
+        for (int i = 0; i < NP; ++i)
+            if (p.id[i] < 0 || p.id[i] >= a.n_pages) {
+                bad |= t * 64 + 16 * SUB * i < len;
+                p.id[i] = 0;
+            }
+        return p;
     };
-    // What lies behind the sequence, on no page or behind head_dim is read from a place that exists (page 0, the row's
-    // first channels, the first channels' rows) and does not count: such scores are masked or met by zeros of q, such
-    // values are cleared or their results not written.
     const int head_bytes = page * d;
-    // The lane's offsets are worked out anew for each tile (from a lane number the compiler does not see through): kept
-    // over the loop they are the first thing it spills, and a reload waits for every load in flight.
-    const auto lane_again = [&]() {
-        int x = lane;
-        asm volatile("" : "+v"(x));
-        return x;
+    const auto copy = [&](const uint8_t *codes, int id, int off, uint8_t *to) {
+        const __amdgpu_buffer_rsrc_t rs =
+            __builtin_amdgcn_make_buffer_rsrc((void *)(codes + ((int64_t)id * a.n_kv_heads + head_kv) * head_bytes), 0, head_bytes, 0x00020000);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, GQ_LDS_PTR(void, to), 16, off, 0, 0, 0);
     };
-    const auto k_offset = [&](int l, int c) {
-        const int mm = l & 15, gg = l >> 4;
-        return (unsigned)((mm & 3) * d + (ONE ? 16 * (mm >> 2) * d : 0) + (64 * c + 16 * gg < d ? 64 * c + 16 * gg : 0));
+    uint8_t *buf_k = sm_k[wave], *buf_v = sm_v[wave];
+    // Copy j brings the pieces 64 j .. 64 j + 63 of the buffer, lane l piece l: of its 128 bytes R the piece that belongs
+    // there.  Channels behind head_dim are out of the descriptor's range and arrive as 0.
+    const auto copy_k = [&](int t, const Pages &p) {
+#pragma unroll
+        for (int j = 0; j < COPIES; ++j) {
+            constexpr int ROWS = 1024 / DP;   // tokens of a copy, all on one page
+            const int piece = (lane & 7) ^ pa_key_swizzle<DP>(8 * j + (lane >> 3));
+            const int row = DP == 128 ? lane >> 3 : 2 * (lane >> 3) + (piece >> 2), ch = 16 * (DP == 128 ? piece : piece & 3);
+            const int tok = (t * 64 + ROWS * j) & (page - 1);
+            const int off = ch < d ? (tok + row) * d + ch : (int)0x80000000;
+            copy(a.k_codes, p.id[ROWS * j / (16 * SUB)], off, buf_k + 1024 * j);
+        }
     };
-    u32x4 kr[4][NC], vr[DT];
+    const auto copy_v = [&](int t, const Pages &p) {
+#pragma unroll
+        for (int j = 0; j < COPIES; ++j) {
+            constexpr int PER = COPIES / NP;   // copies of a page's part of the tile: DP rows of SUB pieces
+            const int q = 64 * (j % PER) + (lane & ~7) + ((lane & 7) ^ (lane >> 3));
+            const int row = q / SUB, tok = ((t * 64 + 16 * SUB * (j / PER)) & (page - 1)) + 16 * (q % SUB);
+            const int off = row < d ? row * page + tok : (int)0x80000000;
+            copy(a.v_codes, p.id[j / PER], off, buf_v + 1024 * j);
+        }
+    };
     float ks, vs, ks_next, vs_next;
-    // ONE: a buffer descriptor of the page's block (scalar), 32-bit lane offsets
-    const auto block_of = [&](const uint8_t *codes, int id) {
-        return __builtin_amdgcn_make_buffer_rsrc((void *)(codes + ((int64_t)id * a.n_kv_heads + head_kv) * head_bytes), 0, head_bytes, 0x00020000);
-    };
-    const auto load_k = [&](int t, int id) {
-        const int l = lane_again();
-        unsigned k_off[NC];
+    const auto load_scales = [&](const Pages &p) {
+        ks_next = pa_scalar_load(a.k_scale, (int64_t)p.id[0] * a.n_kv_heads + head_kv);
+        vs_next = pa_scalar_load(a.v_scale, (int64_t)p.id[0] * a.n_kv_heads + head_kv);
 #pragma unroll
-        for (int c = 0; c < NC; ++c) k_off[c] = k_offset(l, c);
-        if constexpr (ONE) {
-            const pa_rsrc_t rs = block_of(a.k_codes, id);
-            const int at = ((t * 64) & (page - 1)) * d;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int c = 0; c < NC; ++c) kr[i][c] = __builtin_amdgcn_raw_buffer_load_b128(rs, (int)k_off[c], at + 4 * i * d, 0);
-        } else {
-            const uint8_t *p = a.k_codes + ((int64_t)id * a.n_kv_heads + head_kv) * head_bytes + ((t * 64 + 16 * (m >> 2)) & (page - 1)) * d;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int c = 0; c < NC; ++c) kr[i][c] = *reinterpret_cast<const u32x4 *>(p + 4 * i * d + k_off[c]);
+        for (int i = 1; i < NP; ++i) {
+            const int64_t block = (int64_t)p.id[i] * a.n_kv_heads + head_kv;
+            const float k1 = pa_scalar_load(a.k_scale, block), v1 = pa_scalar_load(a.v_scale, block);
+            if (g >= i * SUB) {
+                ks_next = k1;
+                vs_next = v1;
+            }
         }
-    };
-    const auto load_v = [&](int t, int id) {
-        const int l = lane_again();
-        const unsigned v_off = (l & 15) * page + (ONE ? 16 * (l >> 4) : 0);
-        if constexpr (ONE) {
-            const pa_rsrc_t rs = block_of(a.v_codes, id);
-            const int at = (t * 64) & (page - 1);
-#pragma unroll
-            for (int t2 = 0; t2 < DT; ++t2) vr[t2] = __builtin_amdgcn_raw_buffer_load_b128(rs, (int)v_off, at + (16 * t2 < d ? 16 * t2 * page : 0), 0);
-        } else {
-            const uint8_t *p = a.v_codes + ((int64_t)id * a.n_kv_heads + head_kv) * head_bytes + ((t * 64 + 16 * g) & (page - 1));
-#pragma unroll
-            for (int t2 = 0; t2 < DT; ++t2) vr[t2] = *reinterpret_cast<const u32x4 *>(p + (16 * t2 < d ? 16 * t2 * page : 0) + v_off);
-        }
-    };
-    const auto load_scales = [&](int id) {
-        const int64_t block = (int64_t)id * a.n_kv_heads + head_kv;
-        ks_next = a.k_scale[block];
-        vs_next = a.v_scale[block];
     };
 
     f32x4 o[NQ][DT];
@@ -247,47 +254,56 @@ __global__ __launch_bounds__(256, NQ == 1 ? 3 : (NQ == 2 ? 2 : 1)) void attentio
     // tokens from here on are hidden from some row: behind the sequence, or after a query token of it
     const int partly = len - it.n + 1;
 
-    // One set of registers: the next tile's keys are loaded as soon as this one's have met the queries, its values after
-    // this one's have met the weights.
     int t = t_lo + wave;
-    Pages next = {0, 0};
+    Pages next;
+#pragma unroll
+    for (int i = 0; i < NP; ++i) next.id[i] = 0;
     if (t < t_hi) {
         const Pages first = check_pages(fetch_pages(t), t);
+        copy_k(t, first);
+        copy_v(t, first);
+        load_scales(first);
         if (t + 4 < t_hi) next = fetch_pages(t + 4);
-        load_k(t, first.k);
-        load_v(t, first.v);
-        load_scales(first.v);
     }
-    const auto step = [&](auto masked) {
-        const bool more = t + 4 < t_hi;
+    const auto step = [&](auto masked, auto go_on) {
+        const bool more = go_on || t + 4 < t_hi;
         ks = ks_next;
         vs = vs_next;
         Pages now = next;
         if (t + 8 < t_hi) next = fetch_pages(t + 8);
+        // the keys are there: the values' copies may still be under way
+        pa_wait<COPIES>();
         f32x4 s[NQ][4];
 #pragma unroll
         for (int nt = 0; nt < NQ; ++nt)
 #pragma unroll
             for (int i = 0; i < 4; ++i) s[nt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int c = 0; c < NC; ++c)
+        for (int c = 0; c < NC; ++c) {
+            u32x4 kr[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int row = 16 * (m >> 2) + 4 * i + (m & 3), R = DP == 128 ? row : row >> 1, piece = DP == 128 ? 4 * c + g : 4 * (row & 1) + g;
+                kr[i] = *reinterpret_cast<const u32x4 *>(buf_k + 128 * R + 16 * (piece ^ pa_key_swizzle<DP>(R)));
+            }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 vec qf[NQ];
 #pragma unroll
-                for (int nt = 0; nt < NQ; ++nt) qf[nt] = *reinterpret_cast<const vec *>(&sm.q[(16 * nt + m) * QROW + 64 * c + 16 * g + 8 * h]);
+                for (int nt = 0; nt < NQ; ++nt) qf[nt] = *reinterpret_cast<const vec *>(&sm_q[(16 * nt + m) * QROW + 64 * c + 16 * g + 8 * h]);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const vec kf = MM::decode(kr[i][c][2 * h], kr[i][c][2 * h + 1]);
+                    const vec kf = MM::decode(kr[i][2 * h], kr[i][2 * h + 1]);
 #pragma unroll
                     for (int nt = 0; nt < NQ; ++nt) s[nt][i] = MM::run(kf, qf[nt], s[nt][i]);
                 }
-                __builtin_amdgcn_sched_barrier(0);
             }
+        }
         if (more) {
             now = check_pages(now, t + 4);
-            load_k(t + 4, now.k);
-            load_scales(now.v);
+            pa_reads_done();
+            copy_k(t + 4, now);
+            load_scales(now);
         }
         vs = fmaxf(vs, 1e-30f);   // a scale of 0 must not become an infinite weight
         const float mul = a.scale * ks, add = __builtin_amdgcn_logf(vs), inv = 1.f / vs;
@@ -328,6 +344,14 @@ __global__ __launch_bounds__(256, NQ == 1 ? 3 : (NQ == 2 ? 2 : 1)) void attentio
                 }
             l[nt] = fmaf(sum, inv, l[nt]);
         }
+        if (more) pa_wait<COPIES>();   // the values are there: the next keys may be under way
+        else pa_wait<0>();
+        u32x4 vr[DT];
+#pragma unroll
+        for (int t2 = 0; t2 < DT; ++t2) {
+            const int q = (16 * t2 + m) * SUB + g % SUB, R = q >> 3;
+            vr[t2] = *reinterpret_cast<const u32x4 *>(buf_v + (g / SUB) * (DP * SUB * 16) + 128 * R + 16 * ((q & 7) ^ (R & 7)));
+        }
         bool apart = false;   // a NaN among the values of a tile that is not visible to every row
         if (masked) {
             const int left = len - (t * 64 + 16 * g);   // of this lane's 16 tokens
@@ -354,7 +378,6 @@ __global__ __launch_bounds__(256, NQ == 1 ? 3 : (NQ == 2 ? 2 : 1)) void attentio
 #pragma unroll
                     for (int nt = 0; nt < NQ; ++nt) o[nt][t2] = Mfma<_Float16>::run(vf, p[nt][u], o[nt][t2]);
                 }
-                __builtin_amdgcn_sched_barrier(0);
             }
         } else {
             // 0 * NaN is NaN: one token at a time, added only to the rows that see it
@@ -375,13 +398,19 @@ __global__ __launch_bounds__(256, NQ == 1 ? 3 : (NQ == 2 ? 2 : 1)) void attentio
                 }
             }
         }
-        if (more) load_v(t + 4, now.v);
+        if (more) {
+            pa_reads_done();
+            copy_v(t + 4, now);
+        }
+        t += 4;
     };
-    // (kept in order: left to itself the scheduler decodes a whole tile ahead and spills)
-    for (; t < t_hi && (t + 1) * 64 <= partly; t += 4) step(std::false_type());
-    for (; t < t_hi; t += 4) step(std::true_type());
+    // (the first loop without a branch around the copies: a wait the compiler adds has to know what is under way)
+    while ((t + 1) * 64 <= partly && t + 4 < t_hi) step(std::false_type(), std::true_type());
+    while (t < t_hi) step(std::true_type(), std::false_type());
 
-    // join the four waves
+    // join the four waves, through the keys' buffers: a row's 16-byte pieces are permuted by the row, for the banks
+    float *sm_o = reinterpret_cast<float *>(&sm_k[0][0]);
+    const auto o_at = [&](int w, int row, int ch) { return reinterpret_cast<f32x4 *>(sm_o + (w * 16 + row) * DP + 4 * ((ch >> 2) ^ (row & 7))); };
     const bool any_bad = __any(bad);
 #pragma unroll
     for (int nt = 0; nt < NQ; ++nt) {
@@ -399,13 +428,13 @@ __global__ __launch_bounds__(256, NQ == 1 ? 3 : (NQ == 2 ? 2 : 1)) void attentio
         const int rm = 16 * nt + m;
         const float all = fmaxf(fmaxf(sm_m[0][rm], sm_m[1][rm]), fmaxf(sm_m[2][rm], sm_m[3][rm]));
         const float f = mx[nt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx[nt] - all);
-        if (nt > 0) __syncthreads();   // (before the first, all waves are done with the queries)
+        if (nt > 0) __syncthreads();   // (before the first, all waves are done with their tiles)
 #pragma unroll
         for (int t2 = 0; t2 < DT; ++t2) {
             f32x4 x = o[nt][t2];
 #pragma unroll
             for (int j = 0; j < 4; ++j) x[j] *= f;
-            *reinterpret_cast<f32x4 *>(&sm.o[wave][m * LROW + 16 * t2 + 4 * g]) = x;
+            *o_at(wave, m, 16 * t2 + 4 * g) = x;
         }
         __syncthreads();
         const int row = threadIdx.x >> 4, rr = 16 * nt + row, r = it.tile * MR + rr, tok = r / a.group;
@@ -417,7 +446,7 @@ __global__ __launch_bounds__(256, NQ == 1 ? 3 : (NQ == 2 ? 2 : 1)) void attentio
         const int64_t qrow = it.row0 + tok;
         for (int ch = 4 * (threadIdx.x & 15); ch < d; ch += 64) {
             f32x4 x = {0.f, 0.f, 0.f, 0.f};
-            for (int w = 0; w < 4; ++w) x += *reinterpret_cast<const f32x4 *>(&sm.o[w][row * LROW + ch]);
+            for (int w = 0; w < 4; ++w) x += *o_at(w, row, ch);
             if (a.n_splits > 1) {
                 *reinterpret_cast<f32x4 *>(a.part_o + ((qrow * a.n_heads + head) * a.n_splits + split) * d + ch) = x;
             } else {
@@ -534,10 +563,11 @@ template <typename T>
 int launch_paged(const PagedArgs &a, const Plan &p, hipStream_t s)
 {
     const dim3 grid((unsigned)(p.n_items * a.n_kv_heads), (unsigned)p.n_splits);
-#define GQ_PA(NC, NQ)                                                                                                   \
-    do {                                                                                                                \
-        if (a.page_log2 >= 6) hipLaunchKernelGGL((attention_paged_kernel<T, NC, NQ, true>), grid, dim3(256), 0, s, a);  \
-        else hipLaunchKernelGGL((attention_paged_kernel<T, NC, NQ, false>), grid, dim3(256), 0, s, a);                  \
+#define GQ_PA(NC, NQ)                                                                                                       \
+    do {                                                                                                                    \
+        if (a.page_log2 >= 6) hipLaunchKernelGGL((attention_paged_kernel<T, NC, NQ, 4>), grid, dim3(256), 0, s, a);         \
+        else if (a.page_log2 == 5) hipLaunchKernelGGL((attention_paged_kernel<T, NC, NQ, 2>), grid, dim3(256), 0, s, a);    \
+        else hipLaunchKernelGGL((attention_paged_kernel<T, NC, NQ, 1>), grid, dim3(256), 0, s, a);                          \
     } while (0)
     if (a.head_dim <= 64) {
         if (p.nq == 1) GQ_PA(1, 1);
