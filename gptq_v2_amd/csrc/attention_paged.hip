@@ -123,10 +123,11 @@ __device__ __forceinline__ Item find_item(const PagedArgs &a, int item, int mr)
     return {lo, (int)tile, row0, (int)n};
 }
 
-// The place of piece p (of 16 bytes) of the 128 bytes R of a buffer: pieces that are read together lie in different banks.
-// Values are read 8 rows in order; keys in two runs of 4 rows, 16 apart.
+// Piece p (of 16 bytes) of the 128 bytes R of a buffer lies in place p ^ swizzle(R).  16 lanes read 16 pieces at a time
+// over 256 bytes of banks: of 16 adjacent channels' values, of the keys of tokens 16 b + 4 i + 0..3 (b = 0..3).
 template <int DP>
-__device__ __forceinline__ int pa_key_swizzle(int R) { return DP == 128 ? (R & 3) | ((R >> 2) & 4) : (R & 1) | ((R >> 2) & 2); }
+__device__ __forceinline__ int pa_key_swizzle(int R) { return DP == 128 ? ((R >> 1) & 1) | ((R >> 3) & 6) : (R >> 3) & 3; }
+__device__ __forceinline__ int pa_value_swizzle(int R) { return (R >> 1) & 3; }
 
 // SUB: 16-token groups of a tile on one page (pages of 16, 32 and 64 or more: 1, 2, 4)
 template <typename T, int NC, int NQ, int SUB>
@@ -221,7 +222,7 @@ __global__ __launch_bounds__(256, NQ == 4 ? 1 : 2) void attention_paged_kernel(c
 #pragma unroll
         for (int j = 0; j < COPIES; ++j) {
             constexpr int PER = COPIES / NP;   // copies of a page's part of the tile: DP rows of SUB pieces
-            const int q = 64 * (j % PER) + (lane & ~7) + ((lane & 7) ^ (lane >> 3));
+            const int q = 64 * (j % PER) + (lane & ~7) + ((lane & 7) ^ pa_value_swizzle(lane >> 3));
             const int row = q / SUB, tok = ((t * 64 + 16 * SUB * (j / PER)) & (page - 1)) + 16 * (q % SUB);
             const int off = row < d ? row * page + tok : (int)0x80000000;
             copy(a.v_codes, p.id[j / PER], off, buf_v + 1024 * j);
@@ -350,7 +351,7 @@ __global__ __launch_bounds__(256, NQ == 4 ? 1 : 2) void attention_paged_kernel(c
 #pragma unroll
         for (int t2 = 0; t2 < DT; ++t2) {
             const int q = (16 * t2 + m) * SUB + g % SUB, R = q >> 3;
-            vr[t2] = *reinterpret_cast<const u32x4 *>(buf_v + (g / SUB) * (DP * SUB * 16) + 128 * R + 16 * ((q & 7) ^ (R & 7)));
+            vr[t2] = *reinterpret_cast<const u32x4 *>(buf_v + (g / SUB) * (DP * SUB * 16) + 128 * R + 16 * ((q & 7) ^ pa_value_swizzle(R)));
         }
         bool apart = false;   // a NaN among the values of a tile that is not visible to every row
         if (masked) {
@@ -410,7 +411,7 @@ __global__ __launch_bounds__(256, NQ == 4 ? 1 : 2) void attention_paged_kernel(c
 
     // join the four waves, through the keys' buffers: a row's 16-byte pieces are permuted by the row, for the banks
     float *sm_o = reinterpret_cast<float *>(&sm_k[0][0]);
-    const auto o_at = [&](int w, int row, int ch) { return reinterpret_cast<f32x4 *>(sm_o + (w * 16 + row) * DP + 4 * ((ch >> 2) ^ (row & 7))); };
+    const auto o_at = [&](int w, int row, int ch) { return reinterpret_cast<f32x4 *>(sm_o + (w * 16 + row) * DP + 4 * ((ch >> 2) ^ row)); };
     const bool any_bad = __any(bad);
 #pragma unroll
     for (int nt = 0; nt < NQ; ++nt) {

@@ -9,7 +9,7 @@
 // operand P^T when the inner index is taken in that order -- the weights go from the first product to the second
 // without leaving their lane, the row's maximum needs one exchange between two lanes.  K and V tiles are copied to LDS
 // by the asynchronous copy, 16-byte chunks permuted within a row (by the row) so that both the row-wise reads of K and
-// the transposing reads of V (4 tokens x 16 channels per 16 lanes) touch all banks evenly.
+// the transposing reads of V (4 tokens x 16 channels per 16 lanes) touch all banks.
 // Rows behind a sequence's end and channels behind head_dim are out of the buffer descriptor's range and arrive as 0.
 //
 // Bound by the matrix core: 4 head_dim flops per visible (query, key) pair, next to one exponential.
@@ -47,10 +47,15 @@ template <> struct Mma<__bf16> {
     static __device__ __forceinline__ f32x16 run(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 };
 
-// swizzle of a row's 16-byte chunks: the 8 rows that are read together spread over the 8 chunks of 128 bytes (rows of
-// 192 bytes alternate between the halves of 128 by themselves, so theirs is over 4)
+// Chunk c (of 16 bytes) of a row lies in place c ^ swizzle(row).  The banks take 256 bytes at a time: 16 lanes that read
+// one chunk each of 16 adjacent rows of K, 32 lanes that read 64 bytes each of 4 adjacent rows of V (measured: with
+// c ^ (row & 7) the former run at half, the latter at a quarter of the rate).  256 bytes are 1 row of 16 chunks, 2 of 8,
+// and rows of 12 begin in 4 different quarters, so the low bits of the row choose the quarter, the next the chunk in it.
 template <int DP>
-__device__ __forceinline__ int ap_swizzle(int row) { return DP == 96 ? (row >> 1) & 3 : row & 7; }
+__device__ __forceinline__ int ap_swizzle(int row)
+{
+    return DP == 128 ? ((row & 3) << 2) | ((row >> 2) & 3) : (DP == 96 ? (row >> 2) & 3 : ((row & 2) << 1) | ((row >> 2) & 3));
+}
 
 template <typename T, int DP>
 __global__ __launch_bounds__(256, 2) void attention_prompt_kernel(const PromptArgs a)
@@ -139,8 +144,6 @@ __global__ __launch_bounds__(256, 2) void attention_prompt_kernel(const PromptAr
     // tiles that some row of this wave sees
     const int my_last = q0 + wave * 32 + 31 < len - 1 ? q0 + wave * 32 + 31 : len - 1;
     const int my_tiles = a.causal ? (my_last + AP_K) / AP_K : n_tiles;
-    // tiles before this one are visible to every row of the wave
-    const int first_masked = a.causal ? (q0 + wave * 32 + 1) / AP_K : len / AP_K;
     const int see = a.causal ? (row < len - 1 ? row : len - 1) : len - 1;   // the last key this row sees
 
     const auto compute = [&](auto masked, int j, const T *tk, const T *tv) {
@@ -156,7 +159,7 @@ __global__ __launch_bounds__(256, 2) void attention_prompt_kernel(const PromptAr
                 s[tb] = Mma<T>::run(kf, qf[st], s[tb]);
             }
         }
-        if (masked && j >= first_masked) {
+        if (masked) {
 #pragma unroll
             for (int tb = 0; tb < 2; ++tb)
 #pragma unroll
@@ -201,48 +204,49 @@ __global__ __launch_bounds__(256, 2) void attention_prompt_kernel(const PromptAr
             }
             return vf;
         };
-        bool apart = false;
-        if (masked && a.causal && j >= first_masked) {
-            // 0 * inf and 0 * NaN are NaN: an infinity or NaN among these values must not reach the rows before it.
-            // Adding one to an exponent field of all ones carries into the sign's place.
-            unsigned found = 0;
-#pragma unroll 1
-            for (int i = lane; i < AP_K * NCH; i += 64) {
-                const u32x4 x = *reinterpret_cast<const u32x4 *>(tv + i * 8);
 #pragma unroll
-                for (int w = 0; w < 4; ++w) found |= (x[w] & 0x7fff7fffu) + Mma<T>::EXPONENT_ONE;
-            }
-            apart = __any((found & 0x80008000u) != 0);
-        }
-        if (!masked || !apart) {
-#pragma unroll
-            for (int t = 0; t < DT; ++t)
+        for (int t = 0; t < DT; ++t) {
+            if constexpr (!masked) {
 #pragma unroll
                 for (int s2 = 0; s2 < 4; ++s2) o[t] = Mma<T>::run(read_v(t, s2), p[s2], o[t]);
-            return;
-        }
-        // one token at a time, added only to the rows that see it
+            } else {
+                // 0 * inf and 0 * NaN are NaN: an infinity or NaN among these values must not reach the rows before it.
+                // Adding one to an exponent field of all ones carries into the sign's place.
+                vec vf[4];
+                unsigned found = 0;
 #pragma unroll
-        for (int s2 = 0; s2 < 4; ++s2)
-#pragma unroll 1
-            for (int tok = 0; tok < 16; ++tok) {
+                for (int s2 = 0; s2 < 4; ++s2) {
+                    vf[s2] = read_v(t, s2);
+                    unsigned x[4];
+                    __builtin_memcpy(x, &vf[s2], 16);
 #pragma unroll
-                for (int t = 0; t < DT; ++t) {
-                    asm volatile("" ::: "memory");   // keep the reads here: held for all tokens they would cost the common path its registers
-                    vec vf = read_v(t, s2);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        if (8 * (i >> 2) + 4 * h + (i & 3) != tok) vf[i] = static_cast<T>(0.f);
-                    f32x16 x;
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) x[r] = 0.f;
-                    x = Mma<T>::run(vf, p[s2], x);
-                    if (j * AP_K + 16 * s2 + tok <= see) {
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) o[t][r] += x[r];
-                    }
+                    for (int w = 0; w < 4; ++w) found |= (x[w] & 0x7fff7fffu) + Mma<T>::EXPONENT_ONE;
                 }
+                if (!__any((found & 0x80008000u) != 0)) {
+#pragma unroll
+                    for (int s2 = 0; s2 < 4; ++s2) o[t] = Mma<T>::run(vf[s2], p[s2], o[t]);
+                    continue;
+                }
+                // one token at a time, added only to the rows that see it
+#pragma unroll
+                for (int s2 = 0; s2 < 4; ++s2)
+#pragma unroll 1
+                    for (int tok = 0; tok < 16; ++tok) {
+                        vec one = vf[s2];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            if (8 * (i >> 2) + 4 * h + (i & 3) != tok) one[i] = static_cast<T>(0.f);
+                        f32x16 x;
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) x[r] = 0.f;
+                        x = Mma<T>::run(one, p[s2], x);
+                        if (j * AP_K + 16 * s2 + tok <= see) {
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) o[t][r] += x[r];
+                        }
+                    }
             }
+        }
     };
 
     stage(0, 0);
