@@ -82,34 +82,26 @@ __global__ __launch_bounds__(256, 2) void attention_prompt_kernel(const PromptAr
     int64_t row0 = 0, n = a.n_tokens;
     int tile = item;
     if (a.cu) {
-        // sequence b's tiles start at item cu[b] / 128 + b: room for all of them without the host knowing the lengths
-        const auto start = [&](int s) { return (int64_t)a.cu[s] / AP_Q + s; };
-        int lo = 0, hi = a.batch - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (start(mid) <= item) lo = mid;
-            else hi = mid - 1;
+        // Sequence b's tiles start at item cu[b] / 128 + b: room for all of them without the host knowing the lengths.
+        // The starts rise, so b is one less than the number of starts up to this item; 64 are looked at at a time.
+        int lo = -1;
+        for (int b0 = 0; b0 < a.batch; b0 += 64) {
+            const bool before = b0 + lane < a.batch && a.cu[b0 + lane] / AP_Q + b0 + lane <= item;
+            const int c = __popcll(__ballot(before));
+            lo += c;
+            if (c < 64) break;
         }
+        if (lo < 0) return;
+        lo = __builtin_amdgcn_readfirstlane(lo);
         row0 = a.cu[lo];
         n = (int64_t)a.cu[lo + 1] - row0;
-        const int64_t t = item - start(lo);
+        const int64_t t = item - (row0 / AP_Q + lo);
         if (row0 < 0 || n <= 0 || row0 + n > a.n_tokens || t < 0 || t * AP_Q >= n) return;
         tile = (int)t;
     }
     const int len = (int)n, q0 = tile * AP_Q;
     const int d = a.head_dim, head_kv = head / a.group;
     const int row = q0 + wave * 32 + col;            // this lane's query row in its sequence
-
-    vec qf[STEPS];
-    {
-        const T *qp = (const T *)a.q + (row0 + (row < len ? row : 0)) * a.q_tok + head * a.q_head;
-#pragma unroll
-        for (int s = 0; s < STEPS; ++s) {
-            u32x4 raw = {0, 0, 0, 0};
-            if (row < len && 16 * s + 8 * h < d) raw = *reinterpret_cast<const u32x4 *>(qp + 16 * s + 8 * h);
-            __builtin_memcpy(&qf[s], &raw, 16);
-        }
-    }
 
     // what each lane copies of a tile: chunk `tid + 256 j` of the tile in LDS, from its row and unswizzled channel
     const unsigned k_row = (unsigned)(a.k_tok * sizeof(T)), v_row = (unsigned)(a.v_tok * sizeof(T));
@@ -132,6 +124,18 @@ __global__ __launch_bounds__(256, 2) void attention_prompt_kernel(const PromptAr
         for (int p = 0; p < PIECES; ++p)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, GQ_LDS_PTR(void, &sm_v[buf][(wave * 64 + 256 * p) * 8]), 16, (int)v_off[p], 0, 0, 0);
     };
+
+    stage(0, 0);
+    vec qf[STEPS];
+    {
+        const T *qp = (const T *)a.q + (row0 + (row < len ? row : 0)) * a.q_tok + head * a.q_head;
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            u32x4 raw = {0, 0, 0, 0};
+            if (row < len && 16 * s + 8 * h < d) raw = *reinterpret_cast<const u32x4 *>(qp + 16 * s + 8 * h);
+            __builtin_memcpy(&qf[s], &raw, 16);
+        }
+    }
 
     f32x16 o[DT];
 #pragma unroll
@@ -249,7 +253,6 @@ __global__ __launch_bounds__(256, 2) void attention_prompt_kernel(const PromptAr
         }
     };
 
-    stage(0, 0);
     // pairs of tiles that are visible to the whole workgroup, then those that may be masked
     const int n_clear = (a.causal ? (q0 + 1) / AP_K : len / AP_K) & ~1;
     int j = 0;
@@ -272,22 +275,30 @@ __global__ __launch_bounds__(256, 2) void attention_prompt_kernel(const PromptAr
     }
 
     l += __shfl_xor(l, 32, 64);
-    if (row >= len) return;
     const float inv = 1.f / l;
-    T *op = (T *)a.out + (row0 + row) * a.o_tok + head * a.o_head;
+    // A lane holds 4 adjacent channels here and there of its row: through LDS (the wave's 32 rows, places as in the tiles),
+    // so that rows are written in whole lines.
+    __syncthreads();
+    T *so = &sm_k[0][0] + wave * 32 * DP;
 #pragma unroll
     for (int t = 0; t < DT; ++t)
 #pragma unroll
         for (int r4 = 0; r4 < 4; ++r4) {
-            const int ch = 32 * t + 8 * r4 + 4 * h;
-            if (ch >= d) continue;
             T y[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) y[i] = static_cast<T>(o[t][4 * r4 + i] * inv);
             u32x2 raw;
             __builtin_memcpy(&raw, y, 8);
-            *reinterpret_cast<u32x2 *>(op + ch) = raw;
+            *reinterpret_cast<u32x2 *>(so + col * DP + (((4 * t + r4) ^ ap_swizzle<DP>(col)) << 3) + 4 * h) = raw;
         }
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i) {
+        const int piece = i * 64 + lane, r = piece / NCH, c = piece - r * NCH;
+        const int out_row = q0 + wave * 32 + r;
+        const u32x4 x = *reinterpret_cast<const u32x4 *>(so + r * DP + ((c ^ ap_swizzle<DP>(r)) << 3));
+        if (out_row < len && 8 * c < d) *reinterpret_cast<u32x4 *>((T *)a.out + (row0 + out_row) * a.o_tok + head * a.o_head + 8 * c) = x;
+    }
 }
 
 template <typename T>
