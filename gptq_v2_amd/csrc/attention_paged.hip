@@ -536,7 +536,7 @@ struct Plan {
 
 // Query rows per workgroup: as many 16-row tiles as a sequence has rows on average, up to 4.  Splits: enough
 // workgroups to fill the chip, runs of at least 256 tokens (one tile per wave), at most 64 of them.
-Plan paged_plan(int64_t n_tokens, int64_t batch, bool ragged, int n_heads, int n_kv_heads, int page, int64_t table_width)
+Plan paged_plan(int64_t n_tokens, int64_t batch, bool ragged, int64_t n_heads, int64_t n_kv_heads, int64_t page, int64_t table_width)
 {
     Plan p;
     const int64_t group = n_heads / n_kv_heads;
@@ -553,7 +553,7 @@ Plan paged_plan(int64_t n_tokens, int64_t batch, bool ragged, int n_heads, int n
     return p;
 }
 
-bool paged_sizes_ok(int64_t n_tokens, int64_t batch, int n_heads, int n_kv_heads, int head_dim, int page, int64_t table_width)
+bool paged_sizes_ok(int64_t n_tokens, int64_t batch, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim, int64_t page, int64_t table_width)
 {
     return n_tokens >= 0 && n_tokens < ((int64_t)1 << 31) && batch >= 0 && batch < (1 << 24) && n_kv_heads > 0 && n_heads > 0 && n_heads <= 65536 &&
            n_heads % n_kv_heads == 0 && head_dim >= 16 && head_dim <= 128 && head_dim % 16 == 0 &&
@@ -598,25 +598,30 @@ extern "C" size_t gq_attention_paged_workspace(int64_t n_tokens, int64_t batch, 
     return p.n_splits == 1 ? 0 : (size_t)n_tokens * n_heads * p.n_splits * (head_dim + 4) * sizeof(float);
 }
 
-extern "C" int gq_attention_paged(void *out, int64_t out_token_stride, int64_t out_head_stride, const void *q, int64_t q_token_stride,
-                                  int64_t q_head_stride, int dtype, int64_t n_tokens, int n_heads, const void *k_codes, const void *v_codes,
-                                  const float *k_scale, const float *v_scale, int64_t n_pages, int n_kv_heads, int page, int head_dim,
-                                  const int32_t *block_table, int64_t table_width, const int32_t *seq_lens, const int32_t *cu_seqlens,
-                                  int64_t batch, float softmax_scale, void *workspace, size_t workspace_bytes, gq_stream_t stream)
+extern "C" int gq_attention_paged(const gq_attention_paged_args *args, gq_stream_t stream)
 {
-    GQ_REQUIRE(dtype == GQ_F16 || dtype == GQ_BF16, "gq_attention_paged: dtype %d is neither fp16 (0) nor bf16 (1)", dtype);
+    GQ_REQUIRE(args, "gq_attention_paged: NULL pointer");
+    const gq_paged_cache cache = args->cache;
+    const gq_rows out = args->out, q = args->q;
+    const int64_t dtype = args->dtype, n_tokens = args->n_tokens, n_heads = args->n_heads, n_pages = cache.n_pages, n_kv_heads = cache.n_kv_heads;
+    const int64_t page = cache.page, head_dim = cache.head_dim, table_width = args->table_width, batch = args->batch;
+    const int32_t *block_table = args->block_table, *seq_lens = args->seq_lens, *cu_seqlens = args->cu_seqlens;
+    const float softmax_scale = (float)args->softmax_scale;
+    void *workspace = args->workspace;
+    const size_t workspace_bytes = args->workspace_bytes < 0 ? 0 : (size_t)args->workspace_bytes;
+    GQ_REQUIRE(dtype == GQ_F16 || dtype == GQ_BF16, "gq_attention_paged: dtype %lld is neither fp16 (0) nor bf16 (1)", (long long)dtype);
     GQ_REQUIRE(paged_sizes_ok(n_tokens, batch, n_heads, n_kv_heads, head_dim, page, table_width) && n_pages >= 0,
-               "gq_attention_paged: %d heads on %d, head_dim %d (a multiple of 16 up to 128), pages of %d (16, 32, 64 or 128): not supported", n_heads,
-               n_kv_heads, head_dim, page);
+               "gq_attention_paged: %lld heads on %lld, head_dim %lld (a multiple of 16 up to 128), pages of %lld (16, 32, 64 or 128): not supported",
+               (long long)n_heads, (long long)n_kv_heads, (long long)head_dim, (long long)page);
     GQ_REQUIRE(cu_seqlens || n_tokens == batch, "gq_attention_paged: %lld tokens for %lld sequences need cu_seqlens", (long long)n_tokens,
                (long long)batch);
     GQ_REQUIRE(softmax_scale > 0.f && softmax_scale < INFINITY, "gq_attention_paged: the softmax scale must be positive and finite");
     if (n_tokens == 0 || batch == 0) return GQ_OK;
-    GQ_REQUIRE(out && q && seq_lens && (table_width == 0 || block_table) && k_codes && v_codes && k_scale && v_scale,
+    GQ_REQUIRE(out.data && q.data && seq_lens && (table_width == 0 || block_table) && cache.k_codes && cache.v_codes && cache.k_scale && cache.v_scale,
                "gq_attention_paged: NULL pointer");
-    GQ_REQUIRE(q_token_stride % 8 == 0 && q_head_stride % 8 == 0 && out_token_stride % 8 == 0 && out_head_stride % 8 == 0,
+    GQ_REQUIRE(q.token_stride % 8 == 0 && q.head_stride % 8 == 0 && out.token_stride % 8 == 0 && out.head_stride % 8 == 0,
                "gq_attention_paged: strides must be multiples of 8 elements");
-    GQ_REQUIRE((((uintptr_t)out | (uintptr_t)q | (uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)workspace) & 15) == 0,
+    GQ_REQUIRE((((uintptr_t)out.data | (uintptr_t)q.data | (uintptr_t)cache.k_codes | (uintptr_t)cache.v_codes | (uintptr_t)workspace) & 15) == 0,
                "gq_attention_paged: pointers must be 16-byte aligned");
     const Plan p = paged_plan(n_tokens, batch, cu_seqlens != nullptr, n_heads, n_kv_heads, page, table_width);
     GQ_REQUIRE(n_pages > 0, "gq_attention_paged: a cache without pages");
@@ -627,13 +632,13 @@ extern "C" int gq_attention_paged(void *out, int64_t out_token_stride, int64_t o
         return GQ_EWORKSPACE;
     }
     PagedArgs a;
-    a.q = q, a.out = out, a.q_tok = q_token_stride, a.q_head = q_head_stride, a.o_tok = out_token_stride, a.o_head = out_head_stride;
-    a.k_codes = (const uint8_t *)k_codes, a.v_codes = (const uint8_t *)v_codes, a.k_scale = k_scale, a.v_scale = v_scale;
+    a.q = q.data, a.out = out.data, a.q_tok = q.token_stride, a.q_head = q.head_stride, a.o_tok = out.token_stride, a.o_head = out.head_stride;
+    a.k_codes = (const uint8_t *)cache.k_codes, a.v_codes = (const uint8_t *)cache.v_codes, a.k_scale = cache.k_scale, a.v_scale = cache.v_scale;
     a.table = block_table, a.lens = seq_lens, a.cu = cu_seqlens;
     a.part_o = (float *)workspace;
     a.part_ml = (float *)workspace + (size_t)n_tokens * n_heads * p.n_splits * head_dim;
     a.n_tokens = n_tokens, a.n_pages = (int)n_pages, a.table_width = (int)table_width;
-    a.batch = (int)batch, a.n_heads = n_heads, a.n_kv_heads = n_kv_heads, a.group = n_heads / n_kv_heads, a.head_dim = head_dim;
+    a.batch = (int)batch, a.n_heads = (int)n_heads, a.n_kv_heads = (int)n_kv_heads, a.group = (int)(n_heads / n_kv_heads), a.head_dim = (int)head_dim;
     a.page_log2 = __builtin_ctz((unsigned)page), a.tiles_per_split = p.tiles_per_split, a.n_splits = p.n_splits, a.n_items = (int)p.n_items;
     a.scale = softmax_scale * PA_LOG2E;
     return dtype == GQ_F16 ? launch_paged<_Float16>(a, p, (hipStream_t)stream) : launch_paged<__bf16>(a, p, (hipStream_t)stream);

@@ -319,33 +319,37 @@ int launch_prompt(const PromptArgs &a, hipStream_t s)
 
 }  // namespace
 
-extern "C" int gq_attention_prompt(void *out, int64_t out_token_stride, int64_t out_head_stride, const void *q, int64_t q_token_stride,
-                                   int64_t q_head_stride, const void *k, int64_t k_token_stride, int64_t k_head_stride, const void *v,
-                                   int64_t v_token_stride, int64_t v_head_stride, int dtype, int64_t n_tokens, int n_heads, int n_kv_heads,
-                                   int head_dim, const int32_t *cu_seqlens, int64_t batch, int causal, float softmax_scale, gq_stream_t stream)
+extern "C" int gq_attention_prompt(const gq_attention_prompt_args *args, gq_stream_t stream)
 {
-    GQ_REQUIRE(dtype == GQ_F16 || dtype == GQ_BF16, "gq_attention_prompt: dtype %d is neither fp16 (0) nor bf16 (1)", dtype);
-    GQ_REQUIRE(head_dim >= 8 && head_dim <= 128 && head_dim % 8 == 0, "gq_attention_prompt: head_dim %d is not a multiple of 8 up to 128", head_dim);
-    GQ_REQUIRE(n_heads > 0 && n_kv_heads > 0 && n_heads % n_kv_heads == 0 && n_heads <= 65536, "gq_attention_prompt: %d query heads on %d", n_heads, n_kv_heads);
+    GQ_REQUIRE(args, "gq_attention_prompt: NULL pointer");
+    const gq_rows out = args->out, q = args->q, k = args->k, v = args->v;
+    const int64_t dtype = args->dtype, n_tokens = args->n_tokens, n_heads = args->n_heads, n_kv_heads = args->n_kv_heads, head_dim = args->head_dim;
+    const int64_t batch = args->batch;
+    const int32_t *cu_seqlens = args->cu_seqlens;
+    const float softmax_scale = (float)args->softmax_scale;
+    GQ_REQUIRE(dtype == GQ_F16 || dtype == GQ_BF16, "gq_attention_prompt: dtype %lld is neither fp16 (0) nor bf16 (1)", (long long)dtype);
+    GQ_REQUIRE(head_dim >= 8 && head_dim <= 128 && head_dim % 8 == 0, "gq_attention_prompt: head_dim %lld is not a multiple of 8 up to 128", (long long)head_dim);
+    GQ_REQUIRE(n_heads > 0 && n_kv_heads > 0 && n_heads % n_kv_heads == 0 && n_heads <= 65536, "gq_attention_prompt: %lld query heads on %lld",
+               (long long)n_heads, (long long)n_kv_heads);
     GQ_REQUIRE(n_tokens >= 0 && n_tokens < ((int64_t)1 << 30) && batch >= 0 && batch < (1 << 24), "gq_attention_prompt: bad number of tokens or sequences");
     GQ_REQUIRE(cu_seqlens || batch == 1 || n_tokens == 0, "gq_attention_prompt: %lld sequences need cu_seqlens", (long long)batch);
     GQ_REQUIRE(softmax_scale > 0.f && softmax_scale < INFINITY, "gq_attention_prompt: the softmax scale must be positive and finite");
     if (n_tokens == 0 || batch == 0) return GQ_OK;
-    GQ_REQUIRE(out && q && k && v, "gq_attention_prompt: NULL pointer");
-    GQ_REQUIRE(out_token_stride % 8 == 0 && out_head_stride % 8 == 0 && q_token_stride % 8 == 0 && q_head_stride % 8 == 0 && k_token_stride % 8 == 0 &&
-                   k_head_stride % 8 == 0 && v_token_stride % 8 == 0 && v_head_stride % 8 == 0,
+    GQ_REQUIRE(out.data && q.data && k.data && v.data, "gq_attention_prompt: NULL pointer");
+    GQ_REQUIRE(out.token_stride % 8 == 0 && out.head_stride % 8 == 0 && q.token_stride % 8 == 0 && q.head_stride % 8 == 0 && k.token_stride % 8 == 0 &&
+                   k.head_stride % 8 == 0 && v.token_stride % 8 == 0 && v.head_stride % 8 == 0,
                "gq_attention_prompt: strides must be multiples of 8 elements");
     // a tile of 64 rows is addressed by 32-bit offsets, and a row must lie behind the one before it
-    GQ_REQUIRE(n_tokens == 1 || (k_token_stride >= head_dim && v_token_stride >= head_dim && k_token_stride <= (1 << 23) && v_token_stride <= (1 << 23)),
+    GQ_REQUIRE(n_tokens == 1 || (k.token_stride >= head_dim && v.token_stride >= head_dim && k.token_stride <= (1 << 23) && v.token_stride <= (1 << 23)),
                "gq_attention_prompt: token strides of k and v must be in head_dim..2^23");
-    GQ_REQUIRE((((uintptr_t)out | (uintptr_t)q | (uintptr_t)k | (uintptr_t)v) & 15) == 0, "gq_attention_prompt: pointers must be 16-byte aligned");
+    GQ_REQUIRE((((uintptr_t)out.data | (uintptr_t)q.data | (uintptr_t)k.data | (uintptr_t)v.data) & 15) == 0, "gq_attention_prompt: pointers must be 16-byte aligned");
     const int64_t n_items = cu_seqlens ? n_tokens / AP_Q + batch : gq_cdiv(n_tokens, AP_Q);
     GQ_REQUIRE(n_items * n_heads < ((int64_t)1 << 31), "gq_attention_prompt: too many tokens for one call");
     PromptArgs a;
-    a.q = q, a.k = k, a.v = v, a.out = out;
-    a.q_tok = q_token_stride, a.q_head = q_head_stride, a.k_tok = k_token_stride, a.k_head = k_head_stride;
-    a.v_tok = v_token_stride, a.v_head = v_head_stride, a.o_tok = out_token_stride, a.o_head = out_head_stride;
-    a.cu = cu_seqlens, a.n_tokens = n_tokens, a.batch = (int)batch, a.n_heads = n_heads, a.group = n_heads / n_kv_heads;
-    a.head_dim = head_dim, a.n_items = (int)n_items, a.causal = causal != 0, a.scale = softmax_scale * AP_LOG2E;
+    a.q = q.data, a.k = k.data, a.v = v.data, a.out = out.data;
+    a.q_tok = q.token_stride, a.q_head = q.head_stride, a.k_tok = k.token_stride, a.k_head = k.head_stride;
+    a.v_tok = v.token_stride, a.v_head = v.head_stride, a.o_tok = out.token_stride, a.o_head = out.head_stride;
+    a.cu = cu_seqlens, a.n_tokens = n_tokens, a.batch = (int)batch, a.n_heads = (int)n_heads, a.group = (int)(n_heads / n_kv_heads);
+    a.head_dim = (int)head_dim, a.n_items = (int)n_items, a.causal = args->causal != 0, a.scale = softmax_scale * AP_LOG2E;
     return dtype == GQ_F16 ? launch_prompt<_Float16>(a, (hipStream_t)stream) : launch_prompt<__bf16>(a, (hipStream_t)stream);
 }

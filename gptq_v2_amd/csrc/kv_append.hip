@@ -311,43 +311,49 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const AppendArgs a)
 
 }  // namespace
 
-extern "C" int gq_kv_append(void *k_codes, void *v_codes, float *k_scale, float *v_scale, int64_t n_pages, int n_kv_heads, int page,
-                            int head_dim, const void *k, int64_t k_token_stride, int64_t k_head_stride, const void *v, int64_t v_token_stride,
-                            int64_t v_head_stride, int dtype, int64_t n_tokens, const int32_t *block_table, int64_t table_width,
-                            const int32_t *past_lens, const int32_t *cu_seqlens, int64_t batch, const void *q, int64_t q_token_stride,
-                            int64_t q_head_stride, int n_heads, void *q_out, int64_t q_out_token_stride, int64_t q_out_head_stride,
-                            const float *cos_t, const float *sin_t, int64_t max_pos, int rotary_dim, int interleaved, gq_stream_t stream)
+extern "C" int gq_kv_append(const gq_kv_append_args *args, gq_stream_t stream)
 {
-    GQ_REQUIRE(dtype == GQ_F16 || dtype == GQ_BF16, "gq_kv_append: dtype %d is neither fp16 (0) nor bf16 (1)", dtype);
-    GQ_REQUIRE(head_dim >= 16 && head_dim <= 128 && head_dim % 16 == 0, "gq_kv_append: head_dim %d is not a multiple of 16 up to 128", head_dim);
-    GQ_REQUIRE(page == 16 || page == 32 || page == 64 || page == 128, "gq_kv_append: pages of %d tokens: 16, 32, 64 or 128 are supported", page);
+    GQ_REQUIRE(args, "gq_kv_append: NULL pointer");
+    const gq_paged_cache cache = args->cache;
+    const gq_rows k = args->k, v = args->v, q = args->q, q_out = args->q_out;
+    const int64_t dtype = args->dtype, n_tokens = args->n_tokens, n_heads = args->n_heads, n_pages = cache.n_pages, n_kv_heads = cache.n_kv_heads;
+    const int64_t page = cache.page, head_dim = cache.head_dim, table_width = args->table_width, batch = args->batch, max_pos = args->max_pos;
+    const int64_t rotary_dim = args->rotary_dim;
+    const int32_t *block_table = args->block_table, *past_lens = args->past_lens, *cu_seqlens = args->cu_seqlens;
+    const float *cos_t = args->cos, *sin_t = args->sin;
+    GQ_REQUIRE(dtype == GQ_F16 || dtype == GQ_BF16, "gq_kv_append: dtype %lld is neither fp16 (0) nor bf16 (1)", (long long)dtype);
+    GQ_REQUIRE(head_dim >= 16 && head_dim <= 128 && head_dim % 16 == 0, "gq_kv_append: head_dim %lld is not a multiple of 16 up to 128",
+               (long long)head_dim);
+    GQ_REQUIRE(page == 16 || page == 32 || page == 64 || page == 128, "gq_kv_append: pages of %lld tokens: 16, 32, 64 or 128 are supported",
+               (long long)page);
     GQ_REQUIRE(n_kv_heads > 0 && n_pages >= 0 && n_tokens >= 0 && batch >= 0 && table_width >= 0, "gq_kv_append: negative size");
     GQ_REQUIRE(batch < (1 << 24) && n_tokens < ((int64_t)1 << 31) && n_kv_heads <= 65536 && n_heads <= 65536, "gq_kv_append: too many tokens, sequences or heads");
     GQ_REQUIRE(cu_seqlens || n_tokens == batch, "gq_kv_append: %lld tokens for %lld sequences need cu_seqlens", (long long)n_tokens, (long long)batch);
-    GQ_REQUIRE(rotary_dim >= 0 && rotary_dim <= head_dim && rotary_dim % 16 == 0, "gq_kv_append: rotary_dim %d is not a multiple of 16 up to head_dim", rotary_dim);
+    GQ_REQUIRE(rotary_dim >= 0 && rotary_dim <= head_dim && rotary_dim % 16 == 0, "gq_kv_append: rotary_dim %lld is not a multiple of 16 up to head_dim",
+               (long long)rotary_dim);
     if (n_tokens == 0 || batch == 0) return GQ_OK;
-    GQ_REQUIRE(k_codes && v_codes && k_scale && v_scale && k && v && block_table && past_lens, "gq_kv_append: NULL pointer");
+    GQ_REQUIRE(cache.k_codes && cache.v_codes && cache.k_scale && cache.v_scale && k.data && v.data && block_table && past_lens, "gq_kv_append: NULL pointer");
     GQ_REQUIRE(!rotary_dim || (cos_t && sin_t && max_pos > 0), "gq_kv_append: a rotation needs the tables of cosines and sines");
-    GQ_REQUIRE(!q || (q_out && n_heads > 0 && rotary_dim), "gq_kv_append: q needs an output, heads and a rotation");
-    GQ_REQUIRE(k_token_stride % 8 == 0 && k_head_stride % 8 == 0 && v_token_stride % 8 == 0 && v_head_stride % 8 == 0 &&
-                   (!q || (q_token_stride % 8 == 0 && q_head_stride % 8 == 0 && q_out_token_stride % 8 == 0 && q_out_head_stride % 8 == 0)),
+    GQ_REQUIRE(!q.data || (q_out.data && n_heads > 0 && rotary_dim), "gq_kv_append: q needs an output, heads and a rotation");
+    GQ_REQUIRE(k.token_stride % 8 == 0 && k.head_stride % 8 == 0 && v.token_stride % 8 == 0 && v.head_stride % 8 == 0 &&
+                   (!q.data || (q.token_stride % 8 == 0 && q.head_stride % 8 == 0 && q_out.token_stride % 8 == 0 && q_out.head_stride % 8 == 0)),
                "gq_kv_append: strides must be multiples of 8 elements");
-    GQ_REQUIRE((((uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q | (uintptr_t)q_out | (uintptr_t)cos_t |
+    GQ_REQUIRE((((uintptr_t)cache.k_codes | (uintptr_t)cache.v_codes | (uintptr_t)k.data | (uintptr_t)v.data | (uintptr_t)q.data | (uintptr_t)q_out.data | (uintptr_t)cos_t |
                  (uintptr_t)sin_t) & 15) == 0, "gq_kv_append: pointers must be 16-byte aligned");
     AppendArgs a;
-    a.q = q, a.k = k, a.v = v, a.q_out = q_out;
-    a.q_tok = q_token_stride, a.q_head = q_head_stride, a.qo_tok = q_out_token_stride, a.qo_head = q_out_head_stride;
-    a.k_tok = k_token_stride, a.k_head = k_head_stride, a.v_tok = v_token_stride, a.v_head = v_head_stride;
-    a.k_codes = (uint8_t *)k_codes, a.v_codes = (uint8_t *)v_codes, a.k_scale = k_scale, a.v_scale = v_scale;
+    a.q = q.data, a.k = k.data, a.v = v.data, a.q_out = q_out.data;
+    a.q_tok = q.token_stride, a.q_head = q.head_stride, a.qo_tok = q_out.token_stride, a.qo_head = q_out.head_stride;
+    a.k_tok = k.token_stride, a.k_head = k.head_stride, a.v_tok = v.token_stride, a.v_head = v.head_stride;
+    a.k_codes = (uint8_t *)cache.k_codes, a.v_codes = (uint8_t *)cache.v_codes, a.k_scale = cache.k_scale, a.v_scale = cache.v_scale;
     a.cos_t = cos_t, a.sin_t = sin_t, a.table = block_table, a.past = past_lens, a.cu = cu_seqlens;
     a.n_tokens = n_tokens, a.max_pos = max_pos, a.n_pages = n_pages, a.table_width = table_width;
-    a.batch = (int)batch, a.n_heads = n_heads, a.n_kv_heads = n_kv_heads, a.head_dim = head_dim, a.page = page;
-    a.rot = rotary_dim, a.interleaved = interleaved != 0;
+    a.batch = (int)batch, a.n_heads = (int)n_heads, a.n_kv_heads = (int)n_kv_heads, a.head_dim = (int)head_dim, a.page = (int)page;
+    a.rot = (int)rotary_dim, a.interleaved = args->interleaved != 0;
     const int64_t n_items = cu_seqlens ? n_tokens / page + 2 * batch : batch;
     // one wave where a workgroup has a single token (or a small page) to look after
-    const int items_per_page = (cu_seqlens ? page / 4 : 1) * (head_dim / 8);
+    const int64_t items_per_page = (cu_seqlens ? page / 4 : 1) * (head_dim / 8);
     const int threads = items_per_page <= 64 ? 64 : (items_per_page <= 128 ? 128 : 256);
-    const int64_t q_blocks = q ? n_tokens * gq_cdiv(n_heads, threads / (head_dim / 8)) : 0;
+    const int64_t q_blocks = q.data ? n_tokens * gq_cdiv(n_heads, threads / (head_dim / 8)) : 0;
     const int64_t grid = n_items * n_kv_heads * 2 + q_blocks;
     GQ_REQUIRE(grid < ((int64_t)1 << 31), "gq_kv_append: too many tokens for one call");
     a.n_items = (int)n_items;

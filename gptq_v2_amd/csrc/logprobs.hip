@@ -277,14 +277,21 @@ int launch_logprobs(const void *logits, int64_t n_rows, int64_t row_stride, int6
 
 }  // namespace
 
-extern "C" int gq_token_logprobs(const void *logits, int dtype, int64_t n_rows, int64_t row_stride, int64_t vocab, const int64_t *tokens,
-                                 int64_t ignore_index, float *logprob, float *entropy, int top, float *top_logprob, int64_t *top_token,
-                                 gq_stream_t stream)
+extern "C" int gq_token_logprobs(const gq_token_logprobs_args *args, gq_stream_t stream)
 {
-    GQ_REQUIRE(dtype == GQ_F16 || dtype == GQ_BF16 || dtype == GQ_F32, "gq_token_logprobs: dtype %d is none of fp16 (0), bf16 (1), fp32 (2)", dtype);
+    GQ_REQUIRE(args, "gq_token_logprobs: NULL pointer");
+    const void *logits = args->logits;
+    const int64_t dtype = args->dtype, n_rows = args->n_rows, row_stride = args->row_stride, vocab = args->vocab, ignore_index = args->ignore_index;
+    const int64_t *tokens = args->tokens;
+    float *logprob = args->logprob, *entropy = args->entropy, *top_logprob = args->top_logprob;
+    int64_t *top_token = args->top_token;
+    GQ_REQUIRE(dtype == GQ_F16 || dtype == GQ_BF16 || dtype == GQ_F32, "gq_token_logprobs: dtype %lld is none of fp16 (0), bf16 (1), fp32 (2)",
+               (long long)dtype);
     GQ_REQUIRE(n_rows >= 0 && n_rows < ((int64_t)1 << 31), "gq_token_logprobs: bad row count %lld", (long long)n_rows);
     GQ_REQUIRE(vocab > 0 && vocab <= (1 << 30), "gq_token_logprobs: vocab must be in 1..2^30");
-    GQ_REQUIRE(top >= 0 && top <= LP_MAX_TOP && top <= vocab, "gq_token_logprobs: %d alternatives: 0..%d of the vocabulary can be asked for", top, LP_MAX_TOP);
+    GQ_REQUIRE(args->top >= 0 && args->top <= LP_MAX_TOP && args->top <= vocab, "gq_token_logprobs: %lld alternatives: 0..%d of the vocabulary can be asked for",
+               (long long)args->top, LP_MAX_TOP);
+    const int top = (int)args->top;
     GQ_REQUIRE(row_stride >= vocab || n_rows <= 1, "gq_token_logprobs: rows of %lld overlap at a stride of %lld", (long long)vocab, (long long)row_stride);
     if (n_rows == 0) return GQ_OK;
     GQ_REQUIRE(logits && tokens && logprob && entropy && (top == 0 || (top_logprob && top_token)), "gq_token_logprobs: NULL pointer");

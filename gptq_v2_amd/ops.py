@@ -6,6 +6,7 @@ PyTorch is used for device memory and streams only; every function validates its
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import NamedTuple, Optional, Sequence, Tuple
 
 import torch
@@ -667,27 +668,37 @@ def _table(t: torch.Tensor, like: torch.Tensor) -> Tuple[int, int]:
     return shape
 
 
-def _launch(name: str, like: torch.Tensor, *args) -> None:
-    """The C entry `name` on the device and current stream of `like`."""
+def _launch(name: str, like: torch.Tensor, packed: bytes) -> None:
+    """The C entry `name` with its packed argument struct, on the device and current stream of `like`."""
     fn = getattr(_lib.load(), name)
     dev = like.get_device()
     if torch._C._cuda_getDevice() == dev:
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+        rc = fn(packed, torch._C._cuda_getCurrentRawStream(dev))
     else:
         with torch.cuda.device(dev):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+            rc = fn(packed, torch._C._cuda_getCurrentRawStream(dev))
     if rc:
         _lib.check(rc, name)
 
 
+# the argument structs of gptq_amd.h: 8-byte fields (q: a pointer or an integer, d: a double)
+_PROMPT_ARGS = struct.Struct("20qd")
+_APPEND_ARGS = struct.Struct("33q")
+_PAGED_ARGS = struct.Struct("22qd2q")
+_LOGPROBS_ARGS = struct.Struct("12q")
+
+
 def _of(t: Optional[torch.Tensor]):
-    """pointer, token stride, head stride"""
-    return (t.data_ptr(), t.stride(0), t.stride(1)) if t is not None else (None, 0, 0)
+    """struct gq_rows: pointer, token stride, head stride"""
+    if t is None:
+        return 0, 0, 0
+    st = t.stride()
+    return t.data_ptr(), st[0], st[1]
 
 
 def _out_like(out: Optional[torch.Tensor], q: torch.Tensor) -> torch.Tensor:
     if out is None:
-        return q.new_empty(q.shape)
+        return torch.empty_like(q, memory_format=torch.contiguous_format)
     _rows(out, "out", q)
     if out.shape != q.shape:
         raise ValueError(f"out is {tuple(out.shape)}, q {tuple(q.shape)}")
@@ -709,14 +720,14 @@ def attention_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     tk, kv_heads, dk = k.shape
     if k.shape != v.shape or tk != t or dk != d or kv_heads == 0 or heads % kv_heads:
         raise ValueError(f"q is {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
-    batch, cu = 1, None
+    batch, cu = 1, 0
     if cu_seqlens is not None:
         batch = cu_seqlens.numel() - 1 if isinstance(cu_seqlens, torch.Tensor) else 0
         _ints(cu_seqlens, "cu_seqlens", (batch + 1,), q)
         cu = cu_seqlens.data_ptr()
     out = _out_like(out, q)
-    _launch("gq_attention_prompt", q, *_of(out), *_of(q), *_of(k), *_of(v), code, t, heads, kv_heads, d, cu, batch, causal,
-            d ** -0.5 if scale is None else scale)
+    _launch("gq_attention_prompt", q, _PROMPT_ARGS.pack(*_of(out), *_of(q), *_of(k), *_of(v), code, t, heads, kv_heads, d, cu, batch, bool(causal),
+                                                        d ** -0.5 if scale is None else scale))
     return out
 
 
@@ -740,7 +751,7 @@ def kv_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, block_table: 
         raise ValueError(f"k is {tuple(k.shape)}, v {tuple(v.shape)}, the cache has {heads} heads of {d}")
     batch, width = _table(block_table, k)
     _ints(past_lens, "past_lens", (batch,), k)
-    cu = cos_p = sin_p = None
+    cu = cos_p = sin_p = 0
     if cu_seqlens is not None:
         _ints(cu_seqlens, "cu_seqlens", (batch + 1,), k)
         cu = cu_seqlens.data_ptr()
@@ -767,9 +778,9 @@ def kv_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, block_table: 
         q_out = _out_like(q_out, q)
     elif q_out is not None:
         raise ValueError("q_out without q")
-    _launch("gq_kv_append", k, cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), n_pages, heads, page, d,
-            *_of(k), *_of(v), code, t, block_table.data_ptr(), width, past_lens.data_ptr(), cu, batch, *_of(q), n_heads, *_of(q_out), cos_p, sin_p,
-            max_pos, rot, interleaved)
+    _launch("gq_kv_append", k, _APPEND_ARGS.pack(
+        cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), n_pages, heads, page, d, *_of(k), *_of(v), *_of(q),
+        *_of(q_out), code, t, n_heads, block_table.data_ptr(), width, past_lens.data_ptr(), cu, batch, cos_p, sin_p, max_pos, rot, bool(interleaved)))
     return q_out
 
 
@@ -789,18 +800,18 @@ def attention_paged(q: torch.Tensor, cache: PagedCache, block_table: torch.Tenso
         raise ValueError(f"q is {tuple(q.shape)}, the cache has {kv_heads} heads of {d}")
     batch, width = _table(block_table, q)
     _ints(seq_lens, "seq_lens", (batch,), q)
-    cu = None
+    cu = 0
     if cu_seqlens is not None:
         _ints(cu_seqlens, "cu_seqlens", (batch + 1,), q)
         cu = cu_seqlens.data_ptr()
     elif t != batch:
         raise ValueError(f"{t} query tokens for {batch} sequences need cu_seqlens")
     out = _out_like(out, q)
-    need = _lib.load().gq_attention_paged_workspace(t, batch, cu is not None, heads, kv_heads, d, page, width)
+    need = _lib.load().gq_attention_paged_workspace(t, batch, cu != 0, heads, kv_heads, d, page, width)
     ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    _launch("gq_attention_paged", q, *_of(out), *_of(q), code, t, heads, cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
-            cache.v_scale.data_ptr(), n_pages, kv_heads, page, d, block_table.data_ptr(), width, seq_lens.data_ptr(), cu, batch,
-            d ** -0.5 if scale is None else scale, ws.data_ptr() if need else None, need)
+    _launch("gq_attention_paged", q, _PAGED_ARGS.pack(
+        cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), n_pages, kv_heads, page, d, *_of(out), *_of(q), code, t,
+        heads, block_table.data_ptr(), width, seq_lens.data_ptr(), cu, batch, d ** -0.5 if scale is None else scale, ws.data_ptr() if need else 0, need))
     return out
 
 
@@ -828,11 +839,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, ign
         rows, stride = rows.contiguous(), vocab
     if not tokens.is_contiguous():
         tokens = tokens.contiguous()
-    lp = torch.empty(shape, dtype=torch.float32, device=logits.device)
-    ent = torch.empty_like(lp)
+    lp, ent = torch.empty((2, *shape), dtype=torch.float32, device=logits.device).unbind(0)
     tlp = tok = None
     if top:
-        tlp, tok = lp.new_empty((*shape, top)), tokens.new_empty((*shape, top))
-    _launch("gq_token_logprobs", logits, rows.data_ptr(), code, n, stride, vocab, tokens.data_ptr(), ignore_index, lp.data_ptr(), ent.data_ptr(), top,
-            tlp.data_ptr() if top else None, tok.data_ptr() if top else None)
+        tlp, tok = lp.new_empty((*shape, top)), torch.empty((*shape, top), dtype=torch.int64, device=logits.device)
+    _launch("gq_token_logprobs", logits, _LOGPROBS_ARGS.pack(rows.data_ptr(), code, n, stride, vocab, tokens.data_ptr(), ignore_index, lp.data_ptr(),
+                                                             ent.data_ptr(), top, tlp.data_ptr() if top else 0, tok.data_ptr() if top else 0))
     return TokenLogprobs(lp, ent, tlp, tok)

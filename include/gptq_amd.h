@@ -408,21 +408,38 @@ int gq_rope_inplace(void *x, int64_t row_stride, const void *cos_t, const void *
  * cu_seqlens[b] <= i < cu_seqlens[b + 1] (int32, batch + 1 of them, rising).  Rows behind cu_seqlens[batch] are neither
  * read nor written.  Such tensors are given by a token and a head stride in elements (multiples of 8, 16-byte aligned
  * pointers), so that q, k and v may be slices of one merged product.  Query head h reads kv head h / (n_heads / n_kv_heads).
- *
- * gq_attention_prompt: out = softmax(softmax_scale q k^T) v within each sequence; causal != 0: query i sees keys 0..i.
- * cu_seqlens NULL: one sequence of n_tokens (batch 1).  head_dim a multiple of 8 up to 128, sums and softmax in fp32, the
- * weights rounded to `dtype` for the second product. */
-int gq_attention_prompt(void *out, int64_t out_token_stride, int64_t out_head_stride, const void *q, int64_t q_token_stride,
-                        int64_t q_head_stride, const void *k, int64_t k_token_stride, int64_t k_head_stride, const void *v,
-                        int64_t v_token_stride, int64_t v_head_stride, int dtype, int64_t n_tokens, int n_heads, int n_kv_heads,
-                        int head_dim, const int32_t *cu_seqlens, int64_t batch, int causal, float softmax_scale, gq_stream_t stream);
+ * The arguments of a call stand in a struct of 8-byte fields, read during the call only.
+ */
+typedef struct gq_rows {
+    void *data;
+    int64_t token_stride, head_stride;
+} gq_rows;
 
 /* A paged cache of keys and values in 8 bits: e4m3 (OCP) codes with one scale per (page, kv head) and tensor,
  *   k_codes[n_pages][n_kv_heads][page][head_dim], v_codes[n_pages][n_kv_heads][head_dim][page]  (values by channel),
- *   k_scale, v_scale[n_pages][n_kv_heads] fp32;  value = code * scale.
+ *   k_scale, v_scale[n_pages][n_kv_heads];  value = code * scale.
  * page is 16, 32, 64 or 128 tokens, head_dim a multiple of 16 up to 128.  block_table[batch][table_width] names the pages
- * of each sequence in order; an entry outside 0..n_pages-1 is no page.
- *
+ * of each sequence in order; an entry outside 0..n_pages-1 is no page. */
+typedef struct gq_paged_cache {
+    void *k_codes, *v_codes;
+    float *k_scale, *v_scale;
+    int64_t n_pages, n_kv_heads, page, head_dim;
+} gq_paged_cache;
+
+/*
+ * gq_attention_prompt: out = softmax(softmax_scale q k^T) v within each sequence; causal != 0: query i sees keys 0..i.
+ * cu_seqlens NULL: one sequence of n_tokens (batch 1).  head_dim a multiple of 8 up to 128, sums and softmax in fp32, the
+ * weights rounded to `dtype` for the second product. */
+typedef struct gq_attention_prompt_args {
+    gq_rows out, q, k, v;
+    int64_t dtype, n_tokens, n_heads, n_kv_heads, head_dim;
+    const int32_t *cu_seqlens;
+    int64_t batch, causal;
+    double softmax_scale;
+} gq_attention_prompt_args;
+int gq_attention_prompt(const gq_attention_prompt_args *args, gq_stream_t stream);
+
+/*
  * gq_kv_append writes the new tokens of each sequence behind the past_lens[b] it has: the keys rotated, both in e4m3
  * at the page's scale, 2^e with the smallest e (at least -100) for which the page's finite magnitudes fit 448 2^e.  When a
  * page already holds tokens of the sequence its scale does not fall, and they are re-expressed when it grows.  Infinities
@@ -434,12 +451,18 @@ int gq_attention_prompt(void *out, int64_t out_token_stride, int64_t out_head_st
  * q (may be NULL) is rotated the same way into q_out (may be q), rounded once to `dtype`.
  * A token on no page, or whose position has no row in the tables, is not stored; a query row without an angle is NaN.
  * past_lens[b] < 0: nothing is stored for that sequence. */
-int gq_kv_append(void *k_codes, void *v_codes, float *k_scale, float *v_scale, int64_t n_pages, int n_kv_heads, int page,
-                 int head_dim, const void *k, int64_t k_token_stride, int64_t k_head_stride, const void *v, int64_t v_token_stride,
-                 int64_t v_head_stride, int dtype, int64_t n_tokens, const int32_t *block_table, int64_t table_width,
-                 const int32_t *past_lens, const int32_t *cu_seqlens, int64_t batch, const void *q, int64_t q_token_stride,
-                 int64_t q_head_stride, int n_heads, void *q_out, int64_t q_out_token_stride, int64_t q_out_head_stride,
-                 const float *cos_t, const float *sin_t, int64_t max_pos, int rotary_dim, int interleaved, gq_stream_t stream);
+typedef struct gq_kv_append_args {
+    gq_paged_cache cache;
+    gq_rows k, v, q, q_out;
+    int64_t dtype, n_tokens, n_heads;
+    const int32_t *block_table;
+    int64_t table_width;
+    const int32_t *past_lens, *cu_seqlens;
+    int64_t batch;
+    const float *cos, *sin;
+    int64_t max_pos, rotary_dim, interleaved;
+} gq_kv_append_args;
+int gq_kv_append(const gq_kv_append_args *args, gq_stream_t stream);
 
 /* Attention of each sequence's query tokens over its cached keys and values: the n query tokens of sequence b are the last
  * n of its seq_lens[b], and each sees the keys up to its own position (a row that sees none is 0).  cu_seqlens NULL: one
@@ -448,20 +471,36 @@ int gq_kv_append(void *k_codes, void *v_codes, float *k_scale, float *v_scale, i
  * gq_attention_paged_workspace: bytes of scratch memory a call of these sizes needs (0: none); ragged = cu_seqlens given. */
 size_t gq_attention_paged_workspace(int64_t n_tokens, int64_t batch, int ragged, int n_heads, int n_kv_heads, int head_dim, int page,
                                     int64_t table_width);
-int gq_attention_paged(void *out, int64_t out_token_stride, int64_t out_head_stride, const void *q, int64_t q_token_stride,
-                       int64_t q_head_stride, int dtype, int64_t n_tokens, int n_heads, const void *k_codes, const void *v_codes,
-                       const float *k_scale, const float *v_scale, int64_t n_pages, int n_kv_heads, int page, int head_dim,
-                       const int32_t *block_table, int64_t table_width, const int32_t *seq_lens, const int32_t *cu_seqlens,
-                       int64_t batch, float softmax_scale, void *workspace, size_t workspace_bytes, gq_stream_t stream);
+typedef struct gq_attention_paged_args {
+    gq_paged_cache cache;
+    gq_rows out, q;
+    int64_t dtype, n_tokens, n_heads;
+    const int32_t *block_table;
+    int64_t table_width;
+    const int32_t *seq_lens, *cu_seqlens;
+    int64_t batch;
+    double softmax_scale;
+    void *workspace;
+    int64_t workspace_bytes;
+} gq_attention_paged_args;
+int gq_attention_paged(const gq_attention_paged_args *args, gq_stream_t stream);
 
 /* Per row of logits[n_rows][row_stride] (dtype GQ_F16, GQ_BF16 or GQ_F32; vocab of them count): logprob[row], the log
  * probability of tokens[row] (0 where that is ignore_index, NaN where it is no other word of the vocabulary); entropy[row]
  * in nats; and the `top` (0..32) most likely words with their log probabilities, ties to the lowest index.  -inf is a word
  * that cannot come; a row with NaN or +inf, or of -inf alone, gives NaN (its words are those a stable descending sort puts
  * first).  Sums in fp32. */
-int gq_token_logprobs(const void *logits, int dtype, int64_t n_rows, int64_t row_stride, int64_t vocab, const int64_t *tokens,
-                      int64_t ignore_index, float *logprob, float *entropy, int top, float *top_logprob, int64_t *top_token,
-                      gq_stream_t stream);
+typedef struct gq_token_logprobs_args {
+    const void *logits;
+    int64_t dtype, n_rows, row_stride, vocab;
+    const int64_t *tokens;
+    int64_t ignore_index;
+    float *logprob, *entropy;
+    int64_t top;
+    float *top_logprob;
+    int64_t *top_token;
+} gq_token_logprobs_args;
+int gq_token_logprobs(const gq_token_logprobs_args *args, gq_stream_t stream);
 
 #ifdef __cplusplus
 }
