@@ -1,17 +1,24 @@
 // Log probabilities of given tokens from rows of logits, with the entropy and the most likely alternatives.
 //
-// With m = max x, S = sum e^(x - m) and T = sum (x - m) e^(x - m) over a row:
-//   log p(t) = (x_t - m) - log S,     entropy = log S - T / S.
-// One workgroup takes one row and reads it once: every thread keeps a running (m, S, T) of its own elements and
-// rescales it when m grows (S' = S f, T' = (T + d S) f for d = m - m', f = e^d), the workgroup joins them.
+// In units of log 2, y = x log2 e - M for any reference M near the maximum, S = sum 2^y and T = sum y 2^y over a row:
+//   log p(t) = (y_t - log2 S) ln 2,     entropy = (log2 S - T / S) ln 2.
+// (x times the rounded log2 e minus M is one fused operation, and M the same in both places: no error of M counts.)
+// One workgroup takes one row and reads it once.  Every thread sums over its own elements with a reference of its own, to
+// begin with the maximum of the first elements that its wave sees; it moves (S' = S f, T' = (T + d S) f for d = M - M',
+// f = 2^d) only when an element is 2^8 above it, so that nearly all batches of chunks pass without a rescaling (following
+// the maximum itself, some lane of the wave moves in nearly every one).  The sums cost 8 vector instructions an element,
+// against the 11 that HBM's rate leaves time for.
 //
-// The alternatives need no second pass over the row.  The threads form 64 groups, a group's elements a stripe of the
-// row, and the running maxima give each stripe's best element.  The k-th largest of the 64 bounds the k-th largest of
-// the row from below, and only the k stripes at or above that bound can hold larger elements: those (k / 64 of the row,
-// from the cache) are read again and the few elements at or above the bound ranked by counting.  Elements are compared
-// by (value, -index) in one 64-bit word, so ties go to the lowest index.
+// The alternatives need no second pass over the row.  Every thread knows the largest of its own elements and its chunk.
+// Of 64 groups of threads, the k-th largest of the groups' largest bounds the k-th largest of the row from below, and only
+// threads whose own largest is not below the bound (a dozen of 256) can hold larger ones: their elements are read again,
+// by the whole workgroup, and the few at or above the bound ranked by counting.  Elements are compared by (value, -index)
+// in one 64-bit word, so ties go to the lowest index; a thread's largest counts with the last index of its chunk, which
+// can only lower the bound.
 //
 // Bound by HBM: rows * vocab elements in, a few words out.
+#include <type_traits>
+
 #include "gq_common.h"
 
 namespace {
@@ -19,7 +26,7 @@ namespace {
 constexpr int LP_MAX_TOP = 32;
 constexpr int LP_GROUPS = 64;   // at least LP_MAX_TOP; one wave ranks them
 constexpr int LP_LIST = 1024;   // candidates a workgroup ranks; a row with more takes the exhaustive path
-constexpr float LP_LOG2E = 1.44269504088896340736f;
+constexpr float LP_LOG2E = 1.44269504088896340736f, LP_LN2 = 0.69314718055994530942f;
 
 template <typename T> struct Chunk { static constexpr int N = 16 / sizeof(T); };
 
@@ -50,56 +57,43 @@ __device__ __forceinline__ float lp_value(uint64_t key)
     return __uint_as_float((b & 0x80000000u) ? (b & 0x7fffffffu) : ~b);
 }
 
+// Sums with their reference.  Elements of -inf add nothing.
 struct Stat {
     float m, s, t;
+    __device__ __forceinline__ void move(float to)
+    {
+        const float d = m - to, f = __builtin_amdgcn_exp2f(d);
+        t = s == 0.f ? 0.f : fmaf(d, s, t) * f;
+        s *= f;
+        m = to;
+    }
+    __device__ __forceinline__ void add(float x)
+    {
+        const float y = fmaf(x, LP_LOG2E, -m);
+        const float e = __builtin_amdgcn_exp2f(y);
+        s += e;
+        t = fmaf(fmaxf(y, -160.f), e, t);   // (e is 0 there, y may be -inf)
+    }
 };
 
-// One more element range under a common maximum.  -inf is held apart: e^(-inf - m) is 0 and adds nothing, and a
-// thread that has seen nothing else (m = -inf) must not turn that into NaN.
-__device__ __forceinline__ Stat lp_join(Stat a, Stat b)
+// The reference that belongs to an element; beyond 2e38 (a row of the type's lowest value) it is no longer near it, and
+// such a row comes out as one without a sum, which is taken again
+__device__ __forceinline__ float lp_reference(float x) { return fminf(fmaxf(x * LP_LOG2E, -3.0e38f), 3.0e38f); }
+
+template <int WIDTH>
+__device__ __forceinline__ float lp_max(float x)
 {
-    const float m = fmaxf(a.m, b.m);
-    if (m == -INFINITY) return {m, a.s + b.s, 0.f};   // the sums are 0, or NaN from a NaN element
-    const float da = a.m - m, db = b.m - m;
-    const float fa = __builtin_amdgcn_exp2f(da * LP_LOG2E), fb = __builtin_amdgcn_exp2f(db * LP_LOG2E);
-    const float ta = a.m == -INFINITY ? 0.f : fmaf(da, a.s, a.t) * fa;
-    const float tb = b.m == -INFINITY ? 0.f : fmaf(db, b.s, b.t) * fb;
-    return {m, a.s * fa + b.s * fb, ta + tb};
+#pragma unroll
+    for (int off = WIDTH / 2; off > 0; off >>= 1) x = fmaxf(x, __shfl_xor(x, off, 64));
+    return x;
 }
 
-__device__ __forceinline__ Stat lp_shuffle(Stat a, int off)
+template <int WIDTH>
+__device__ __forceinline__ float lp_sum(float x)
 {
-    return {__shfl_xor(a.m, off, 64), __shfl_xor(a.s, off, 64), __shfl_xor(a.t, off, 64)};
-}
-
-template <int N>
-__device__ __forceinline__ void lp_take(const float (&x)[N], uint32_t index, Stat &st, uint32_t &best)
-{
-    float cm = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-        cm = fmaxf(cm, x[i]);
-    if (cm > st.m || best == 0xffffffffu) {
-        int at = 0;
-#pragma unroll
-        for (int i = N - 1; i >= 0; --i)
-            if (x[i] == cm) at = i;
-        best = index + at;
-        if (st.m != -INFINITY) {
-            const float d = st.m - cm, f = __builtin_amdgcn_exp2f(d * LP_LOG2E);
-            st.t = fmaf(d, st.s, st.t) * f;
-            st.s *= f;
-        }
-        st.m = cm;
-    }
-    const float ref = st.m == -INFINITY ? 0.f : st.m;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const float d = x[i] - ref;
-        const float e = __builtin_amdgcn_exp2f(d * LP_LOG2E);
-        st.s += e;
-        st.t = fmaf(fmaxf(d, -3.0e38f), e, st.t);   // -inf * 0 counts as 0
-    }
+    for (int off = WIDTH / 2; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
+    return x;
 }
 
 template <typename T, int NT>
@@ -109,15 +103,15 @@ __global__ __launch_bounds__(NT) void token_logprobs_kernel(const T *__restrict_
                                                             float *__restrict__ top_logprob, int64_t *__restrict__ top_token)
 {
     constexpr int VEC = Chunk<T>::N;
-    constexpr int UNROLL = 4;
+    constexpr int UNROLL = 2;
     constexpr int WAVES = NT / 64;
     constexpr int PER_GROUP = NT / LP_GROUPS;
     __shared__ float sm_m[WAVES], sm_s[WAVES], sm_t[WAVES];
     __shared__ uint64_t sm_best[NT];
     __shared__ uint64_t sm_list[LP_LIST];
     __shared__ uint64_t sm_bound;
-    __shared__ int sm_stripe[LP_MAX_TOP];
-    __shared__ int sm_count;
+    __shared__ int sm_thread[NT];
+    __shared__ int sm_threads, sm_count;
 
     const int64_t row = blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -129,109 +123,169 @@ __global__ __launch_bounds__(NT) void token_logprobs_kernel(const T *__restrict_
     const int tail0 = head + n_chunks * VEC;
     const T *xc = x + head;
 
-    Stat st = {-INFINITY, 0.f, 0.f};
-    uint32_t best = 0xffffffffu;
-    if (tid < head) {
-        const float one[1] = {static_cast<float>(x[tid])};
-        lp_take<1>(one, tid, st, best);
-    }
-    int c = tid;
-    for (; c + (UNROLL - 1) * NT < n_chunks; c += UNROLL * NT) {
-        float f[UNROLL][VEC];
-#pragma unroll
-        for (int u = 0; u < UNROLL; ++u) load_chunk(xc + (int64_t)(c + u * NT) * VEC, f[u]);
-#pragma unroll
-        for (int u = 0; u < UNROLL; ++u) lp_take<VEC>(f[u], head + (c + u * NT) * VEC, st, best);
-    }
-    for (; c < n_chunks; c += NT) {
-        float f[VEC];
-        load_chunk(xc + (int64_t)c * VEC, f);
-        lp_take<VEC>(f, head + c * VEC, st, best);
-    }
-    if (tid < vocab - tail0) {
-        const float one[1] = {static_cast<float>(x[tail0 + tid])};
-        lp_take<1>(one, tail0 + tid, st, best);
+    int64_t token = 0;
+    float x_token = 0.f;
+    if (tid == 0) {
+        token = tokens[row];
+        if (token >= 0 && token < vocab) x_token = static_cast<float>(x[token]);
     }
 
+    Stat st = {-3.0e38f, 0.f, 0.f};
+    float best = -INFINITY;   // of this thread's chunks, and the chunk it is in
+    int best_at = -1;
+    const auto take = [&](int c, auto whole) {
+        float f[UNROLL][VEC];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            if (whole || c + u * NT < n_chunks) {
+                load_chunk(xc + (c + u * NT) * VEC, f[u]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) f[u][i] = -INFINITY;
+            }
+        }
+        float most = -INFINITY;   // (a maximum passes over NaN)
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            float of_chunk = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) of_chunk = fmaxf(of_chunk, f[u][i]);
+            if ((whole || c + u * NT < n_chunks) && (of_chunk > best || best_at < 0)) {
+                best = of_chunk;
+                best_at = c + u * NT;
+            }
+            most = fmaxf(most, of_chunk);
+        }
+        if (c < NT) st.m = lp_reference(lp_max<64>(most));   // the first batch
+        const float m = lp_reference(most);
+        if (__any(m > st.m + 8.f)) st.move(fmaxf(m, st.m));
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) st.add(f[u][i]);
+    };
+    int c0 = 0;
+    for (; c0 + UNROLL * NT <= n_chunks; c0 += UNROLL * NT) take(c0 + tid, std::true_type());
+    if (c0 < n_chunks) take(c0 + tid, std::false_type());
+    // the elements before the first and behind the last chunk
+    if (tid < head + (vocab - tail0)) {
+        const float v = static_cast<float>(x[tid < head ? tid : tail0 + tid - head]);
+        const float m = lp_reference(v);
+        if (m > st.m + 8.f) st.move(m);
+        st.add(v);
+    }
+
+    const float top_m = lp_max<64>(st.m);
+    if (lane == 0) sm_m[wave] = top_m;
+    const uint64_t own = best_at >= 0 ? lp_key(best, head + best_at * VEC + VEC - 1) : 0;
     if (top > 0) {
-        uint64_t key = best == 0xffffffffu ? 0 : lp_key(st.m, best);
+        uint64_t key = own;
 #pragma unroll
         for (int off = PER_GROUP / 2; off > 0; off >>= 1) {
             const uint64_t o = __shfl_xor((unsigned long long)key, off, 64);
             key = o > key ? o : key;
         }
         if (tid % PER_GROUP == 0) sm_best[tid / PER_GROUP] = key;
-        if (tid == 0) sm_count = 0;
+        if (tid == 0) {
+            sm_count = sm_threads = 0;
+            sm_bound = 0;
+        }
     }
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) st = lp_join(st, lp_shuffle(st, off));
+    __syncthreads();
+    st.move(lp_max<WAVES>(sm_m[lane % WAVES]));
+    st.s = lp_sum<64>(st.s);
+    st.t = lp_sum<64>(st.t);
     if (lane == 0) {
-        sm_m[wave] = st.m;
         sm_s[wave] = st.s;
         sm_t[wave] = st.t;
     }
-    __syncthreads();
-    st = {sm_m[0], sm_s[0], sm_t[0]};
-    for (int w = 1; w < WAVES; ++w) st = lp_join(st, {sm_m[w], sm_s[w], sm_t[w]});
-    // no element, only -inf, a NaN or +inf: not a distribution
-    const bool bad = !(st.m > -INFINITY) || !(st.s > 0.f);
-    const float log_s = bad ? NAN : logf(st.s);
-    if (tid == 0) {
-        const int64_t t = tokens[row];
-        float lp = NAN;
-        if (t == ignore_index) lp = 0.f;
-        else if (t >= 0 && t < vocab) lp = (static_cast<float>(x[t]) - st.m) - log_s;
-        logprob[row] = lp;
-        entropy[row] = log_s - st.t / st.s;
-    }
-    if (top == 0) return;
-
-    // ranks of the groups' best (the words differ, but for the zeros of groups without an element)
-    if (tid < LP_GROUPS) {
+    // the top-th of the groups' largest (the words differ; of fewer groups with an element the bound stays 0)
+    if (top > 0 && tid < LP_GROUPS) {
         const uint64_t mine = sm_best[tid];
         int rank = 0;
-        for (int i = 0; i < LP_GROUPS; ++i) {
-            const uint64_t o = sm_best[i];
-            rank += (o > mine) || (o == mine && i < tid);
-        }
-        if (rank < top) sm_stripe[rank] = tid;
+#pragma unroll 16
+        for (int i = 0; i < LP_GROUPS; ++i) rank += sm_best[i] > mine;
         if (rank == top - 1) sm_bound = mine;
     }
     __syncthreads();
-    const uint64_t bound = sm_bound;
-    const int per_stripe = (n_chunks + NT - 1) / NT * PER_GROUP;
-    for (int i = tid; i < top * per_stripe; i += NT) {
-        const int s = i / per_stripe, j = i - s * per_stripe;
-        const int ch = sm_stripe[s] * PER_GROUP + (j % PER_GROUP) + (j / PER_GROUP) * NT;
-        if (ch >= n_chunks) continue;
-        float f[VEC];
-        load_chunk(xc + (int64_t)ch * VEC, f);
-#pragma unroll
-        for (int j2 = 0; j2 < VEC; ++j2) {
-            const uint64_t key = lp_key(f[j2], head + ch * VEC + j2);
-            if (key >= bound) {
-                const int at = atomicAdd(&sm_count, 1);
-                if (at < LP_LIST) sm_list[at] = key;
-            }
+    st.s = lp_sum<WAVES>(sm_s[lane % WAVES]);
+    st.t = lp_sum<WAVES>(sm_t[lane % WAVES]);
+    // No sum: a row of numbers beyond the reference's range, of -inf alone, with NaN or +inf.  It is taken again, from its
+    // maximum; the last three come out as NaN.
+    float log_s = log2f(st.s), unit = LP_LN2, m = st.m;
+    const bool odd = !(st.s > 0.f && st.s < INFINITY);
+    if (odd) {
+        __syncthreads();
+        float most = -INFINITY;
+        for (int i = tid; i < vocab; i += NT) most = fmaxf(most, static_cast<float>(x[i]));
+        most = lp_max<64>(most);
+        if (lane == 0) sm_m[wave] = most;
+        __syncthreads();
+        m = lp_max<WAVES>(sm_m[lane % WAVES]);
+        float s = 0.f, t = 0.f;
+        for (int i = tid; i < vocab; i += NT) {
+            const float d = static_cast<float>(x[i]) - m, e = __builtin_amdgcn_exp2f(d * LP_LOG2E);
+            s += e;
+            t = fmaf(fmaxf(d, -3.0e38f), e, t);
         }
+        s = lp_sum<64>(s);
+        t = lp_sum<64>(t);
+        if (lane == 0) {
+            sm_s[wave] = s;
+            sm_t[wave] = t;
+        }
+        __syncthreads();
+        st.s = lp_sum<WAVES>(sm_s[lane % WAVES]);
+        st.t = lp_sum<WAVES>(sm_t[lane % WAVES]);
+        log_s = st.s > 0.f ? logf(st.s) : NAN;
+        unit = 1.f;
     }
-    if (tid < head + (vocab - tail0)) {
-        const int idx = tid < head ? tid : tail0 + tid - head;
-        const uint64_t key = lp_key(static_cast<float>(x[idx]), idx);
+    const auto log_p = [&](float v) { return ((odd ? v - m : fmaf(v, LP_LOG2E, -m)) - log_s) * unit; };
+    if (tid == 0) {
+        float lp = NAN;
+        if (token == ignore_index) lp = 0.f;
+        else if (token >= 0 && token < vocab) lp = log_p(x_token);
+        logprob[row] = lp;
+        entropy[row] = (log_s - st.t / st.s) * unit;
+    }
+    if (top == 0) return;
+    const uint64_t bound = sm_bound;
+    const float bound_value = lp_value(bound);   // (a bound of 0 is NaN: below nothing)
+    const auto offer = [&](float v, int index) {
+        if (v < bound_value) return;
+        const uint64_t key = lp_key(v, index);
         if (key >= bound) {
             const int at = atomicAdd(&sm_count, 1);
             if (at < LP_LIST) sm_list[at] = key;
         }
+    };
+    if (own != 0 && own >= bound) sm_thread[atomicAdd(&sm_threads, 1)] = tid;
+    __syncthreads();
+    const int per_thread = (n_chunks + NT - 1) / NT, n_again = sm_threads * per_thread;
+    for (int i = tid; i < n_again; i += NT) {
+        const int s = i / per_thread, ch = sm_thread[s] + (i - s * per_thread) * NT;
+        if (ch >= n_chunks) continue;
+        float g[VEC], most = -INFINITY;
+        load_chunk(xc + ch * VEC, g);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) most = fmaxf(most, g[j]);
+        if (most < bound_value) continue;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) offer(g[j], head + ch * VEC + j);
+    }
+    if (tid < head + (vocab - tail0)) {
+        const int idx = tid < head ? tid : tail0 + tid - head;
+        offer(static_cast<float>(x[idx]), idx);
     }
     __syncthreads();
     const int count = sm_count;
-    if (count <= LP_LIST && !bad) {
+    if (count <= LP_LIST && !odd) {
         for (int i = tid; i < count; i += NT) {
             const uint64_t key = sm_list[i];
             int r = 0;
             for (int j = 0; j < count; ++j) r += sm_list[j] > key;
             if (r < top) {
-                top_logprob[row * top + r] = (lp_value(key) - st.m) - log_s;
+                top_logprob[row * top + r] = log_p(lp_value(key));
                 top_token[row * top + r] = (int64_t)(0xfffffffeu - (uint32_t)key);
             }
         }
@@ -255,7 +309,7 @@ __global__ __launch_bounds__(NT) void token_logprobs_kernel(const T *__restrict_
         last = sm_best[0];
         __syncthreads();
         if (tid == 0) {
-            top_logprob[row * top + r] = bad ? NAN : (lp_value(last) - st.m) - log_s;
+            top_logprob[row * top + r] = log_p(lp_value(last));
             top_token[row * top + r] = (int64_t)(0xfffffffeu - (uint32_t)last);
         }
     }
@@ -268,7 +322,9 @@ int launch_logprobs(const void *logits, int64_t n_rows, int64_t row_stride, int6
 #define GQ_LP(NT)                                                                                                                      \
     hipLaunchKernelGGL((token_logprobs_kernel<T, NT>), dim3((unsigned)n_rows), dim3(NT), 0, s, (const T *)logits, row_stride, (int)vocab, \
                        tokens, ignore_index, logprob, entropy, top, top_logprob, top_token)
-    if (n_rows <= 512) GQ_LP(1024);
+    // 16 waves a row where rows are few and have a chunk or two for each thread (1 x 32000 fp16: 7.8 us), 4 waves where the
+    // rows fill the chip by themselves (4096 x 50272 bf16: 87 us; 8 waves 89, 16 waves 157)
+    if (n_rows <= 512 && vocab * (int64_t)sizeof(T) >= 32768) GQ_LP(1024);
     else GQ_LP(256);
 #undef GQ_LP
     GQ_LAUNCH_CHECK();
