@@ -12,9 +12,11 @@
 // lies in (224, 448]).  Every value is rounded once from 32 bits: the rotated key never passes through 16 bits.
 //
 // One workgroup owns a (sequence's page, kv head, keys or values): it needs the largest magnitude before the first
-// store, and nobody else may touch the page while codes are re-expressed.  A thread holds 4 tokens x 8 channels in
-// registers between the two, so the input is read once where the page has no more than one such item per thread.
-// Bound by HBM for prompts (16-bit input in, one byte out), by launch and two dependent loads for single tokens.
+// store, and nobody else may touch the page while codes are re-expressed.  The input stays in registers between the two.
+// A thread takes 16 channels of each of two tokens of keys -- the two halves of 8 rotated pairs, one angle for both -- or 4
+// tokens x 8 channels of values, whose codes go through LDS so that both the
+// loads (by token) and the stores (by channel) are whole lines.
+// Bound by HBM for prompts (16-bit input in, one byte out), by launch and dependent loads for single tokens.
 #include "gq_common.h"
 
 namespace {
@@ -31,7 +33,7 @@ struct AppendArgs {
     const float *cos_t, *sin_t;       // [max_pos][rot / 2]
     const int32_t *table, *past, *cu;   // cu NULL: one token per sequence
     int64_t n_tokens, max_pos, n_pages, table_width;
-    int batch, n_heads, n_kv_heads, head_dim, page, rot, interleaved, n_items;
+    int batch, n_heads, n_kv_heads, head_dim, page, rot, interleaved, n_items, q_parts;
 };
 
 template <typename T>
@@ -55,35 +57,45 @@ __device__ __forceinline__ void store8f(T *p, const float (&f)[8])
     *reinterpret_cast<u32x4 *>(p) = raw;
 }
 
-// 8 channels of one head at channel c0 < rot after the rotation, each product and the sum rounded in 32 bits
-template <typename T>
-__device__ __forceinline__ void load8_rotated(const T *head, int c0, const float *cos_r, const float *sin_r, int rot, int interleaved,
-                                              float (&f)[8])
+// Pair p of a head: 16 channels as two runs of 8, at `lo` and `hi`.  Of a rotated part in two halves they are partners.
+__device__ __forceinline__ void pair_channels(int p, int rot, int interleaved, int &lo, int &hi)
 {
-    load8f(head + c0, f);
-    if (c0 >= rot) return;
+    const bool halves = !interleaved && 16 * p < rot;
+    lo = halves ? 8 * p : 16 * p;
+    hi = halves ? lo + (rot >> 1) : lo + 8;
+}
+
+// Loads pair p of a head and rotates it by the angles of cos_r / sin_r (rows of the tables; NULL: as it is), each product
+// and the sum rounded in 32 bits.
+template <typename T>
+__device__ __forceinline__ void load_pair(const T *head, int p, const float *cos_r, const float *sin_r, int rot, int interleaved, float (&a)[8],
+                                          float (&b)[8])
+{
+    int lo, hi;
+    pair_channels(p, rot, interleaved, lo, hi);
+    load8f(head + lo, a);
+    load8f(head + hi, b);
+    if (16 * p >= rot) return;
+    // the 8 angles of this pair: of channels (lo + i, hi + i), or of (2 j, 2 j + 1) for j = 8 p + i
+    float c[8], s[8];
+    *reinterpret_cast<f32x4 *>(c) = *reinterpret_cast<const f32x4 *>(cos_r + 8 * p);
+    *reinterpret_cast<f32x4 *>(c + 4) = *reinterpret_cast<const f32x4 *>(cos_r + 8 * p + 4);
+    *reinterpret_cast<f32x4 *>(s) = *reinterpret_cast<const f32x4 *>(sin_r + 8 * p);
+    *reinterpret_cast<f32x4 *>(s + 4) = *reinterpret_cast<const f32x4 *>(sin_r + 8 * p + 4);
+    const auto turn = [](float &x, float &y, float cs, float sn) {
+        const float u = x, v = y;
+        x = __fsub_rn(__fmul_rn(u, cs), __fmul_rn(v, sn));
+        y = __fadd_rn(__fmul_rn(v, cs), __fmul_rn(u, sn));
+    };
     if (interleaved) {
-        const f32x4 c = *reinterpret_cast<const f32x4 *>(cos_r + c0 / 2), s = *reinterpret_cast<const f32x4 *>(sin_r + c0 / 2);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float a = f[2 * i], b = f[2 * i + 1];
-            f[2 * i] = __fsub_rn(__fmul_rn(a, c[i]), __fmul_rn(b, s[i]));
-            f[2 * i + 1] = __fadd_rn(__fmul_rn(b, c[i]), __fmul_rn(a, s[i]));
+            turn(a[2 * i], a[2 * i + 1], c[i], s[i]);
+            turn(b[2 * i], b[2 * i + 1], c[4 + i], s[4 + i]);
         }
     } else {
-        const int half = rot >> 1;
-        const bool low = c0 < half;
-        float o[8];
-        load8f(head + (low ? c0 + half : c0 - half), o);
-        const int r0 = low ? c0 : c0 - half;
-        float c[8], s[8];
-        *reinterpret_cast<f32x4 *>(c) = *reinterpret_cast<const f32x4 *>(cos_r + r0);
-        *reinterpret_cast<f32x4 *>(c + 4) = *reinterpret_cast<const f32x4 *>(cos_r + r0 + 4);
-        *reinterpret_cast<f32x4 *>(s) = *reinterpret_cast<const f32x4 *>(sin_r + r0);
-        *reinterpret_cast<f32x4 *>(s + 4) = *reinterpret_cast<const f32x4 *>(sin_r + r0 + 4);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            f[i] = low ? __fsub_rn(__fmul_rn(f[i], c[i]), __fmul_rn(o[i], s[i])) : __fadd_rn(__fmul_rn(f[i], c[i]), __fmul_rn(o[i], s[i]));
+        for (int i = 0; i < 8; ++i) turn(a[i], b[i], c[i], s[i]);
     }
 }
 
@@ -110,21 +122,23 @@ __device__ __forceinline__ int exponent_for(unsigned bits)
     return e < MIN_EXP ? MIN_EXP : (e > MAX_EXP ? MAX_EXP : e);
 }
 
-// The sequence that `pos` of a rising row of batch + 1 starts lies in: the last b < batch with f(b) <= pos.
+// The sequence that `pos` of a rising row of batch + 1 starts lies in: the last b < batch with f(b) <= pos (-1: none), one
+// less than how many there are; a wave looks at 64 at a time.
 template <typename F>
 __device__ __forceinline__ int find_sequence(int batch, int64_t pos, F f)
 {
-    int lo = 0, hi = batch - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (f(mid) <= pos) lo = mid;
-        else hi = mid - 1;
+    const int lane = threadIdx.x & 63;
+    int n = 0;
+    for (int b0 = 0; b0 < batch; b0 += 64) {
+        const int c = __popcll(__ballot(b0 + lane < batch && f(b0 + lane) <= pos));
+        n += c;
+        if (c < 64) break;
     }
-    return lo;
+    return __builtin_amdgcn_readfirstlane(n) - 1;
 }
 
 template <typename T>
-__device__ __forceinline__ void append_page(const AppendArgs &a, int item, int head, bool is_v, unsigned *sm_max)
+__device__ __forceinline__ void append_page(const AppendArgs &a, int item, int head, bool is_v, unsigned *sm_max, unsigned *sm_tile)
 {
     const int tid = threadIdx.x, nt = blockDim.x;
     int b = item, j = 0;
@@ -133,10 +147,11 @@ __device__ __forceinline__ void append_page(const AppendArgs &a, int item, int h
         // sequence b starts at item cu[b] / page + 2 b: room for the (n + page - 2) / page + 1 pages it can touch
         const auto start = [&](int s) { return (int64_t)a.cu[s] / a.page + 2 * (int64_t)s; };
         b = find_sequence(a.batch, item, start);
+        if (b < 0) return;
         j = (int)(item - start(b));
         row0 = a.cu[b];
         n = (int64_t)a.cu[b + 1] - row0;
-        if (j < 0 || row0 < 0 || n <= 0 || row0 + n > a.n_tokens) return;
+        if (row0 < 0 || n <= 0 || row0 + n > a.n_tokens) return;
     }
     const int64_t past = a.past[b];
     if (past < 0) return;
@@ -149,7 +164,7 @@ __device__ __forceinline__ void append_page(const AppendArgs &a, int item, int h
     const int64_t page_id = a.table[(int64_t)b * a.table_width + pidx];
     if (page_id < 0 || page_id >= a.n_pages) return;
 
-    const int d = a.head_dim, n_ch = d >> 3;
+    const int d = a.head_dim;
     const T *x = is_v ? (const T *)a.v + head * a.v_head : (const T *)a.k + head * a.k_head;
     const int64_t tok_stride = is_v ? a.v_tok : a.k_tok;
     const int64_t block = page_id * a.n_kv_heads + head;
@@ -157,38 +172,48 @@ __device__ __forceinline__ void append_page(const AppendArgs &a, int item, int h
     float *scale = (is_v ? a.v_scale : a.k_scale) + block;
     const float old = *scale;
     const int64_t row_of_0 = row0 + first - past;   // row of the page's slot 0, were it new
-    // items that hold new tokens: quads s0 / 4 .. (s1 - 1) / 4
-    const int quad0 = s0 >> 2, live_quads = ((s1 - 1) >> 2) - quad0 + 1, n_live = live_quads * n_ch;
 
-    float f[4][8];
-    int quad = 0, ch = 0;
-    const auto fetch = [&](int it) {
-        // channels vary fastest for keys (a row is stored whole), tokens for values
-        quad = quad0 + (is_v ? it % live_quads : it / n_ch);
-        ch = is_v ? it / live_quads : it % n_ch;
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            const int s = 4 * quad + t;
-            if (s < s0 || s >= s1) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) f[t][i] = 0.f;
-                continue;
-            }
-            const T *p = x + (row_of_0 + s) * tok_stride;
-            if (is_v || a.rot == 0) load8f(p + 8 * ch, f[t]);
-            else load8_rotated(p, 8 * ch, a.cos_t + (first + s) * (a.rot >> 1), a.sin_t + (first + s) * (a.rot >> 1), a.rot, a.interleaved, f[t]);
-        }
-    };
+    // Items of keys: a token and 16 channels, two for a thread.  Items of values: 4 tokens (of one word of codes) and 8
+    // channels, one for a thread.
+    float f[2][16];   // (f[t / 2][8 (t % 2) ..]: token t of the values)
+    const int n_pairs = d >> 4, n_ch = d >> 3;
+    const int n_keys = (s1 - s0) * n_pairs;
+    const int quad0 = s0 >> 2, n_quads = ((s1 - 1) >> 2) - quad0 + 1, n_vals = n_quads * n_ch;
+    const int quad = quad0 + tid / n_ch, ch = tid % n_ch;
     unsigned most = 0;
-    for (int it = tid; it < n_live; it += nt) {
-        fetch(it);
+    const auto measure = [&](float v) {
+        const unsigned bits = __float_as_uint(v) & 0x7fffffffu;
+        if (bits < 0x7f800000u && bits > most) most = bits;
+    };
+    if (is_v) {
+        if (tid < n_vals) {
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+            for (int t = 0; t < 4; ++t) {
+                float (&g)[8] = *reinterpret_cast<float (*)[8]>(&f[t >> 1][8 * (t & 1)]);
+                const int s = 4 * quad + t;
+                if (s >= s0 && s < s1) {
+                    load8f(x + (row_of_0 + s) * tok_stride + 8 * ch, g);
+                } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const unsigned bits = __float_as_uint(f[t][i]) & 0x7fffffffu;
-                if (bits < 0x7f800000u && bits > most) most = bits;
+                    for (int i = 0; i < 8; ++i) g[i] = 0.f;
+                }
             }
+#pragma unroll
+            for (int k = 0; k < 32; ++k) measure(f[k >> 4][k & 15]);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int it = tid + k * nt;
+            if (it < n_keys) {
+                const int s = s0 + it / n_pairs;
+                const int64_t at = (first + s) * (a.rot >> 1);
+                load_pair(x + (row_of_0 + s) * tok_stride, it % n_pairs, a.cos_t + at, a.sin_t + at, a.rot, a.interleaved,
+                          *reinterpret_cast<float (*)[8]>(&f[k][0]), *reinterpret_cast<float (*)[8]>(&f[k][8]));
+#pragma unroll
+                for (int i = 0; i < 16; ++i) measure(f[k][i]);
+            }
+        }
     }
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) {
@@ -230,82 +255,109 @@ __device__ __forceinline__ void append_page(const AppendArgs &a, int item, int h
     }
     if (tid == 0) *scale = pow2f(e);
     const float inv = pow2f(-e);
-    for (int it = tid; it < n_live; it += nt) {
-        if (n_live > nt) fetch(it);
-        if (is_v) {
-            const bool whole = 4 * quad >= s0 && 4 * quad + 4 <= s1;
+    if (!is_v) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const unsigned w = to_codes4(f[0][i] * inv, f[1][i] * inv, f[2][i] * inv, f[3][i] * inv);
-                uint8_t *p = codes + (8 * ch + i) * a.page + 4 * quad;
-                if (whole) {
-                    *reinterpret_cast<unsigned *>(p) = w;
-                } else {
-#pragma unroll
-                    for (int t = 0; t < 4; ++t)
-                        if (4 * quad + t >= s0 && 4 * quad + t < s1) p[t] = (uint8_t)(w >> (8 * t));
-                }
+        for (int k = 0; k < 2; ++k) {
+            const int it = tid + k * nt;
+            if (it < n_keys) {
+                int lo, hi;
+                pair_channels(it % n_pairs, a.rot, a.interleaved, lo, hi);
+                uint8_t *row = codes + (s0 + it / n_pairs) * d;
+                const float (&g)[16] = f[k];
+                u32x2 w;
+                w[0] = to_codes4(g[0] * inv, g[1] * inv, g[2] * inv, g[3] * inv);
+                w[1] = to_codes4(g[4] * inv, g[5] * inv, g[6] * inv, g[7] * inv);
+                *reinterpret_cast<u32x2 *>(row + lo) = w;
+                w[0] = to_codes4(g[8] * inv, g[9] * inv, g[10] * inv, g[11] * inv);
+                w[1] = to_codes4(g[12] * inv, g[13] * inv, g[14] * inv, g[15] * inv);
+                *reinterpret_cast<u32x2 *>(row + hi) = w;
             }
+        }
+        return;
+    }
+    // A word of 4 tokens of channel c: in LDS at [c][word], the words of a row permuted by its 8 channels' number (16 lanes
+    // with 16 such numbers write side by side); a word that is only partly new goes out by bytes.
+    const int row_words = a.page >> 2;
+    const auto put = [&](int c, int q, unsigned w) {
+        uint8_t *p = codes + c * a.page + 4 * q;
+        if (4 * q >= s0 && 4 * q + 4 <= s1) {
+            *reinterpret_cast<unsigned *>(p) = w;
         } else {
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                const int s = 4 * quad + t;
-                if (s < s0 || s >= s1) continue;
-                u32x2 w;
-                w[0] = to_codes4(f[t][0] * inv, f[t][1] * inv, f[t][2] * inv, f[t][3] * inv);
-                w[1] = to_codes4(f[t][4] * inv, f[t][5] * inv, f[t][6] * inv, f[t][7] * inv);
-                *reinterpret_cast<u32x2 *>(codes + s * d + 8 * ch) = w;
-            }
+            for (int t = 0; t < 4; ++t)
+                if (4 * q + t >= s0 && 4 * q + t < s1) p[t] = (uint8_t)(w >> (8 * t));
+        }
+    };
+    if (tid < n_vals) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const unsigned w = to_codes4(f[0][i] * inv, f[0][8 + i] * inv, f[1][i] * inv, f[1][8 + i] * inv);
+            if (n_quads == 1) put(8 * ch + i, quad, w);
+            else sm_tile[(8 * ch + i) * row_words + (quad ^ (ch & (row_words - 1)))] = w;
+        }
+    }
+    if (n_quads == 1) return;
+    __syncthreads();
+    const int pieces = a.page >> 4;   // of 16 tokens
+    for (int i = tid; i < d * pieces; i += nt) {
+        const int c = i / pieces, q = 4 * (i - c * pieces);
+        u32x4 w;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[k] = sm_tile[c * row_words + ((q + k) ^ ((c >> 3) & (row_words - 1)))];
+        if (4 * q >= s0 && 4 * q + 16 <= s1) {
+            *reinterpret_cast<u32x4 *>(codes + c * a.page + 4 * q) = w;
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (4 * (q + k) < s1 && 4 * (q + k) + 4 > s0) put(c, q + k, w[k]);
         }
     }
 }
 
-// The query rows of one token, a block of heads: a thread takes 8 channels and, where those are the lower half of a
-// rotated pair, their partners too, so that q_out may be q.
+// The query rows of a token, or part of its heads: a thread takes 16 channels, both sides of a rotated pair, so that q_out may be q.
 template <typename T>
-__device__ __forceinline__ void rotate_query(const AppendArgs &a, int64_t token, int head_block)
+__device__ __forceinline__ void rotate_query(const AppendArgs &a, int64_t token, int part)
 {
-    const int n_ch = a.head_dim >> 3, per = blockDim.x / n_ch;
-    const int hl = threadIdx.x / n_ch, ch = threadIdx.x - hl * n_ch, head = head_block * per + hl;
-    if (hl >= per || head >= a.n_heads) return;
     int64_t pos;
     if (a.cu) {
         if (token < a.cu[0] || token >= a.cu[a.batch]) return;   // behind the last sequence: left as it is
         const int b = find_sequence(a.batch, token, [&](int s) { return (int64_t)a.cu[s]; });
+        if (b < 0) return;
         pos = a.past[b] < 0 ? -1 : (int64_t)a.past[b] + (token - a.cu[b]);
     } else {
         pos = a.past[token];
     }
-    const T *x = (const T *)a.q + token * a.q_tok + head * a.q_head;
-    T *y = (T *)a.q_out + token * a.qo_tok + head * a.qo_head;
     const bool known = pos >= 0 && pos < a.max_pos;
-    const int half = a.rot >> 1, c0 = 8 * ch;
-    const float *cr = a.cos_t + (known ? pos : 0) * half, *sr = a.sin_t + (known ? pos : 0) * half;
-    const bool pair = !a.interleaved && c0 < a.rot;
-    if (pair && c0 >= half) return;   // written with its partner
-    float lo[8], hi[8];
-    load8_rotated(x, c0, cr, sr, a.rot, a.interleaved, lo);
-    if (pair) load8_rotated(x, c0 + half, cr, sr, a.rot, 0, hi);
-    if (!known) {
+    const int64_t at = (known ? pos : 0) * (a.rot >> 1);
+    const int n_pairs = a.head_dim >> 4, n = a.n_heads * n_pairs;
+    for (int i = part * blockDim.x + threadIdx.x; i < n; i += a.q_parts * blockDim.x) {
+        const int head = i / n_pairs, p = i - head * n_pairs;
+        float lo[8], hi[8];
+        load_pair((const T *)a.q + token * a.q_tok + head * a.q_head, p, a.cos_t + at, a.sin_t + at, a.rot, a.interleaved, lo, hi);
+        if (!known) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) lo[i] = hi[i] = NAN;
+            for (int k = 0; k < 8; ++k) lo[k] = hi[k] = NAN;
+        }
+        int cl, chh;
+        pair_channels(p, a.rot, a.interleaved, cl, chh);
+        T *y = (T *)a.q_out + token * a.qo_tok + head * a.qo_head;
+        store8f(y + cl, lo);
+        store8f(y + chh, hi);
     }
-    store8f(y + c0, lo);
-    if (pair) store8f(y + c0 + half, hi);
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void kv_append_kernel(const AppendArgs a)
+__global__ __launch_bounds__(512) void kv_append_kernel(const AppendArgs a)
 {
-    __shared__ unsigned sm_max[4];
+    __shared__ unsigned sm_max[8];
+    extern __shared__ unsigned sm_tile[];   // values of a page, where whole words of tokens are new
     const unsigned n_kv = (unsigned)a.n_items * a.n_kv_heads * 2;
     if (blockIdx.x < n_kv) {
         const unsigned ih = blockIdx.x >> 1, item = ih / a.n_kv_heads;
-        append_page<T>(a, (int)item, (int)(ih - item * a.n_kv_heads), blockIdx.x & 1, sm_max);
+        append_page<T>(a, (int)item, (int)(ih - item * a.n_kv_heads), blockIdx.x & 1, sm_max, sm_tile);
     } else {
-        const int per = blockDim.x / (a.head_dim >> 3);
-        const unsigned blocks = (a.n_heads + per - 1) / per, i = blockIdx.x - n_kv;
-        rotate_query<T>(a, i / blocks, (int)(i % blocks));
+        const unsigned i = blockIdx.x - n_kv, token = i / a.q_parts;
+        rotate_query<T>(a, token, (int)(i - token * a.q_parts));
     }
 }
 
@@ -350,15 +402,18 @@ extern "C" int gq_kv_append(const gq_kv_append_args *args, gq_stream_t stream)
     a.batch = (int)batch, a.n_heads = (int)n_heads, a.n_kv_heads = (int)n_kv_heads, a.head_dim = (int)head_dim, a.page = (int)page;
     a.rot = (int)rotary_dim, a.interleaved = args->interleaved != 0;
     const int64_t n_items = cu_seqlens ? n_tokens / page + 2 * batch : batch;
-    // one wave where a workgroup has a single token (or a small page) to look after
-    const int64_t items_per_page = (cu_seqlens ? page / 4 : 1) * (head_dim / 8);
-    const int threads = items_per_page <= 64 ? 64 : (items_per_page <= 128 ? 128 : 256);
-    const int64_t q_blocks = q.data ? n_tokens * gq_cdiv(n_heads, threads / (head_dim / 8)) : 0;
+    // Two 16-channel items of keys for each thread of a page, which is one 4 x 8 item of values; one wave for single tokens.
+    // Queries: an item for each thread where tokens are few, a workgroup for a token where they fill the chip.
+    const int64_t pairs = (cu_seqlens ? page : 1) * (head_dim / 16);
+    const int threads = pairs <= 128 ? 64 : (pairs <= 256 ? 128 : (pairs <= 512 ? 256 : 512));
+    a.q_parts = n_tokens < 1024 ? (int)gq_cdiv(n_heads * (head_dim / 16), threads) : 1;
+    const int64_t q_blocks = q.data ? n_tokens * a.q_parts : 0;
+    const size_t lds = cu_seqlens ? (size_t)(page * head_dim) : 0;
     const int64_t grid = n_items * n_kv_heads * 2 + q_blocks;
     GQ_REQUIRE(grid < ((int64_t)1 << 31), "gq_kv_append: too many tokens for one call");
     a.n_items = (int)n_items;
-    if (dtype == GQ_F16) hipLaunchKernelGGL(kv_append_kernel<_Float16>, dim3((unsigned)grid), dim3(threads), 0, (hipStream_t)stream, a);
-    else hipLaunchKernelGGL(kv_append_kernel<__bf16>, dim3((unsigned)grid), dim3(threads), 0, (hipStream_t)stream, a);
+    if (dtype == GQ_F16) hipLaunchKernelGGL(kv_append_kernel<_Float16>, dim3((unsigned)grid), dim3(threads), lds, (hipStream_t)stream, a);
+    else hipLaunchKernelGGL(kv_append_kernel<__bf16>, dim3((unsigned)grid), dim3(threads), lds, (hipStream_t)stream, a);
     GQ_LAUNCH_CHECK();
     return GQ_OK;
 }
