@@ -85,11 +85,11 @@ SIGNATURES = {
     "gq_xtx_tail_workspace": (c_size_t, [c_int64]),
     "gq_xtx_accumulate_tail": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_void_p]),
     "gq_xtx_fold_tail": (c_int, [c_void_p, c_void_p, c_int64, c_void_p]),
-    "gq_attention_prompt": (c_int, [c_char_p, c_void_p]),    # (the struct's bytes, stream)
-    "gq_kv_append": (c_int, [c_char_p, c_void_p]),
+    "gq_attention_prompt": (c_int, [c_void_p, c_void_p]),    # (address of the struct, stream)
+    "gq_kv_append": (c_int, [c_void_p, c_void_p]),
     "gq_attention_paged_workspace": (c_size_t, [c_int64, c_int64, c_int, c_int, c_int, c_int, c_int, c_int64]),
-    "gq_attention_paged": (c_int, [c_char_p, c_void_p]),
-    "gq_token_logprobs": (c_int, [c_char_p, c_void_p]),
+    "gq_attention_paged": (c_int, [c_void_p, c_void_p]),
+    "gq_token_logprobs": (c_int, [c_void_p, c_void_p]),
     "gq_gemm_nt": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p]),
 }
 

@@ -19,6 +19,22 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=o
          "-I" + os.path.join(ROOT, "include"), "-I" + CSRC, "-Wall", "-Wno-unused-function"]
 
 
+BINDING = os.path.join(HERE, "_serving_binding.so")
+
+
+def _binding_cmd() -> list:
+    """g++ line of the torch-facing binding (csrc/serving_binding.cpp); the C library itself needs no torch headers."""
+    import sysconfig
+    import torch
+    base = os.path.dirname(torch.__file__)
+    lib = os.path.join(base, "lib")
+    return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", "-I" + os.path.join(ROOT, "include"),
+            "-isystem", os.path.join(base, "include"), "-isystem", os.path.join(base, "include", "torch", "csrc", "api", "include"),
+            "-isystem", "/opt/rocm/include", "-isystem", sysconfig.get_paths()["include"], "-Wall", os.path.join(CSRC, "serving_binding.cpp"), "-o", BINDING,
+            "-L" + lib, "-Wl,-rpath," + lib, "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_hip"]
+
+
 def _hipcc() -> str:
     exe = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
     if not os.path.exists(exe):
@@ -54,8 +70,11 @@ def build(force: bool = False, verbose: bool = True) -> str:
             print(" ".join(cmd), flush=True)
         subprocess.check_call(cmd)
 
-    with ThreadPoolExecutor(max_workers=min(8, max(1, len(jobs)))) as ex:
-        list(ex.map(run, jobs))
+    binding = []
+    if force or _stale(BINDING, [os.path.join(CSRC, "serving_binding.cpp"), os.path.join(ROOT, "include", "gptq_amd.h")]):
+        binding = [_binding_cmd()]
+    with ThreadPoolExecutor(max_workers=min(8, max(1, len(jobs) + len(binding)))) as ex:
+        list(ex.map(run, binding + jobs))
     if jobs or force or _stale(LIB, objs):
         run([hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB, *objs])
     return LIB

@@ -6,7 +6,6 @@ PyTorch is used for device memory and streams only; every function validates its
 from __future__ import annotations
 
 import ctypes
-import struct
 from typing import NamedTuple, Optional, Sequence, Tuple
 
 import torch
@@ -609,100 +608,18 @@ class TokenLogprobs(NamedTuple):
     top_token: Optional[torch.Tensor]      # (rows..., top) int64
 
 
-# A decoder's step calls these operators once per layer and token with little work each, so the checks first ask for what is
-# nearly always so, cheaply, and look for the reason only when it is not.
-
-def _no_grad(*ts: Optional[torch.Tensor]) -> None:
-    if torch.is_grad_enabled():
-        for t in ts:
-            if t is not None and t.requires_grad:
-                raise RuntimeError("this operator has no backward pass: call it under torch.no_grad() or on detached tensors")
-
-
-def _rows(t: torch.Tensor, name: str, like: Optional[torch.Tensor] = None) -> None:
-    """A (tokens, heads, head_dim) tensor whose last dimension is dense; the others may have any stride of 8 elements."""
-    if isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 3 and t.stride(2) == 1 and (
-            like is None or t.dtype == like.dtype and t.get_device() == like.get_device()):
-        return
-    if not isinstance(t, torch.Tensor):
-        raise TypeError(f"{name}: expected a tensor")
-    if t.device.type != "cuda":
-        raise ValueError(f"{name}: must live on the GPU (got {t.device}); there is no CPU path")
-    if t.dim() != 3:
-        raise ValueError(f"{name}: expected (tokens, heads, head_dim), got {t.dim()} dimensions")
-    if t.stride(2) != 1:
-        raise ValueError(f"{name}: the last dimension must be contiguous")
-    raise ValueError(f"{name}: is {t.dtype} on {t.device}, expected {like.dtype} on {like.device}")
+def _load_binding():
+    """The C++ binding of these operators (csrc/serving_binding.cpp: checks, outputs and the call, where checks in Python
+    would take longer than the kernels), on the entries of the library that ``_lib`` has loaded."""
+    from . import _serving_binding as b
+    lib = _lib.load()
+    address = lambda name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value  # noqa: E731
+    b.bind(address("gq_attention_prompt"), address("gq_kv_append"), address("gq_attention_paged_workspace"), address("gq_attention_paged"),
+           address("gq_token_logprobs"), lib.gq_version(), _lib.check)
+    return b
 
 
-def _ints(t: torch.Tensor, name: str, shape: Tuple[int, ...], like: torch.Tensor) -> None:
-    if isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.shape == shape and t.get_device() == like.get_device() and t.is_contiguous():
-        return
-    if not isinstance(t, torch.Tensor):
-        raise TypeError(f"{name}: expected a tensor")
-    raise ValueError(f"{name}: expected contiguous int32 {shape} on {like.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-
-
-def _check_cache(cache: PagedCache, like: torch.Tensor) -> Tuple[int, int, int, int]:
-    k, v, ks, vs = cache
-    dev = like.get_device()
-    if (isinstance(k, torch.Tensor) and isinstance(v, torch.Tensor) and isinstance(ks, torch.Tensor) and isinstance(vs, torch.Tensor)
-            and k.dtype is torch.float8_e4m3fn and v.dtype is torch.float8_e4m3fn and ks.dtype is torch.float32 and vs.dtype is torch.float32
-            and k.get_device() == dev and v.get_device() == dev and ks.get_device() == dev and vs.get_device() == dev and k.dim() == 4
-            and k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
-        n_pages, heads, page, d = k.shape
-        if v.shape == (n_pages, heads, d, page) and ks.shape == (n_pages, heads) and vs.shape == (n_pages, heads):
-            return n_pages, heads, page, d
-    for t, name in zip(cache, PagedCache._fields):
-        _check(t, name, torch.float32 if name.endswith("scale") else torch.float8_e4m3fn, 2 if name.endswith("scale") else 4)
-        if t.get_device() != dev:
-            raise ValueError(f"{name}: on {t.device}, expected {like.device}")
-    raise ValueError(f"the cache's tensors do not belong together: {[tuple(t.shape) for t in cache]}")
-
-
-def _table(t: torch.Tensor, like: torch.Tensor) -> Tuple[int, int]:
-    if not isinstance(t, torch.Tensor) or t.dim() != 2:
-        raise ValueError("block_table: expected (sequences, pages)")
-    shape = t.shape
-    _ints(t, "block_table", shape, like)
-    return shape
-
-
-def _launch(name: str, like: torch.Tensor, packed: bytes) -> None:
-    """The C entry `name` with its packed argument struct, on the device and current stream of `like`."""
-    fn = getattr(_lib.load(), name)
-    dev = like.get_device()
-    if torch._C._cuda_getDevice() == dev:
-        rc = fn(packed, torch._C._cuda_getCurrentRawStream(dev))
-    else:
-        with torch.cuda.device(dev):
-            rc = fn(packed, torch._C._cuda_getCurrentRawStream(dev))
-    if rc:
-        _lib.check(rc, name)
-
-
-# the argument structs of gptq_amd.h: 8-byte fields (q: a pointer or an integer, d: a double)
-_PROMPT_ARGS = struct.Struct("20qd")
-_APPEND_ARGS = struct.Struct("33q")
-_PAGED_ARGS = struct.Struct("22qd2q")
-_LOGPROBS_ARGS = struct.Struct("12q")
-
-
-def _of(t: Optional[torch.Tensor]):
-    """struct gq_rows: pointer, token stride, head stride"""
-    if t is None:
-        return 0, 0, 0
-    st = t.stride()
-    return t.data_ptr(), st[0], st[1]
-
-
-def _out_like(out: Optional[torch.Tensor], q: torch.Tensor) -> torch.Tensor:
-    if out is None:
-        return torch.empty_like(q, memory_format=torch.contiguous_format)
-    _rows(out, "out", q)
-    if out.shape != q.shape:
-        raise ValueError(f"out is {tuple(out.shape)}, q {tuple(q.shape)}")
-    return out
+_serving = _load_binding()
 
 
 def attention_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None, causal: bool = True,
@@ -711,24 +628,7 @@ def attention_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     a multiple of 8 up to 128; strided views (slices of a merged q/k/v product) are taken as they are.  ``cu_seqlens``
     (sequences + 1) int32 says where the packed sequences begin and end (None: one sequence); rows behind the last are left
     as they are.  Causal: token i of a sequence sees tokens 0..i.  ``scale`` defaults to head_dim ** -0.5."""
-    _no_grad(q, k, v, out)
-    _rows(q, "q")
-    _rows(k, "k", q)
-    _rows(v, "v", q)
-    code = _dtype_code(q)
-    t, heads, d = q.shape
-    tk, kv_heads, dk = k.shape
-    if k.shape != v.shape or tk != t or dk != d or kv_heads == 0 or heads % kv_heads:
-        raise ValueError(f"q is {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
-    batch, cu = 1, 0
-    if cu_seqlens is not None:
-        batch = cu_seqlens.numel() - 1 if isinstance(cu_seqlens, torch.Tensor) else 0
-        _ints(cu_seqlens, "cu_seqlens", (batch + 1,), q)
-        cu = cu_seqlens.data_ptr()
-    out = _out_like(out, q)
-    _launch("gq_attention_prompt", q, _PROMPT_ARGS.pack(*_of(out), *_of(q), *_of(k), *_of(v), code, t, heads, kv_heads, d, cu, batch, bool(causal),
-                                                        d ** -0.5 if scale is None else scale))
-    return out
+    return _serving.attention_prompt(q, k, v, cu_seqlens, causal, scale, out)
 
 
 def kv_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor, past_lens: torch.Tensor,
@@ -740,48 +640,7 @@ def kv_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, block_table: 
     rotated on the way, and q (tokens, heads, head_dim), if given, into ``q_out`` (which may be q), which is returned; pairs of
     channels are (j, j + rotary_dim / 2), or (2j, 2j + 1) if ``interleaved``.  See gq_kv_append in gptq_amd.h for the scales
     and for tokens without a page or an angle."""
-    _no_grad(k, v, q, q_out)
-    _rows(k, "k")
-    _rows(v, "v", k)
-    code = _dtype_code(k)
-    n_pages, heads, page, d = _check_cache(cache, k)
-    shape = k.shape
-    t = shape[0]
-    if shape != v.shape or shape != (t, heads, d):
-        raise ValueError(f"k is {tuple(k.shape)}, v {tuple(v.shape)}, the cache has {heads} heads of {d}")
-    batch, width = _table(block_table, k)
-    _ints(past_lens, "past_lens", (batch,), k)
-    cu = cos_p = sin_p = 0
-    if cu_seqlens is not None:
-        _ints(cu_seqlens, "cu_seqlens", (batch + 1,), k)
-        cu = cu_seqlens.data_ptr()
-    elif t != batch:
-        raise ValueError(f"{t} tokens for {batch} sequences need cu_seqlens")
-    rot = max_pos = 0
-    if (cos is None) != (sin is None):
-        raise ValueError("cos and sin belong together")
-    if cos is not None:
-        _check(cos, "cos", torch.float32, 2)
-        _check(sin, "sin", torch.float32, 2)
-        if cos.shape != sin.shape or cos.get_device() != k.get_device() or sin.get_device() != k.get_device():
-            raise ValueError(f"cos is {tuple(cos.shape)} on {cos.device}, sin {tuple(sin.shape)} on {sin.device}")
-        max_pos, rot = cos.shape
-        rot, cos_p, sin_p = 2 * rot, cos.data_ptr(), sin.data_ptr()
-    n_heads = 0
-    if q is not None:
-        if not rot:
-            raise ValueError("q is given to be rotated: cos and sin are missing")
-        _rows(q, "q", k)
-        tq, n_heads, dq = q.shape
-        if tq != t or dq != d:
-            raise ValueError(f"q is {tuple(q.shape)}, k {tuple(k.shape)}")
-        q_out = _out_like(q_out, q)
-    elif q_out is not None:
-        raise ValueError("q_out without q")
-    _launch("gq_kv_append", k, _APPEND_ARGS.pack(
-        cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), n_pages, heads, page, d, *_of(k), *_of(v), *_of(q),
-        *_of(q_out), code, t, n_heads, block_table.data_ptr(), width, past_lens.data_ptr(), cu, batch, cos_p, sin_p, max_pos, rot, bool(interleaved)))
-    return q_out
+    return _serving.kv_append(*cache, k, v, block_table, past_lens, cu_seqlens, q, cos, sin, interleaved, q_out)
 
 
 def attention_paged(q: torch.Tensor, cache: PagedCache, block_table: torch.Tensor, seq_lens: torch.Tensor,
@@ -791,28 +650,7 @@ def attention_paged(q: torch.Tensor, cache: PagedCache, block_table: torch.Tenso
     own position.  ``cu_seqlens`` None: one query token for each sequence (a decoder's step); several are a checked
     draft or a chunk of a prompt behind its cached beginning.  A row that sees nothing is 0; a sequence with a token on no page
     is NaN.  The scratch memory of long sequences comes from torch's allocator, a tensor per call."""
-    _no_grad(q, out)
-    _rows(q, "q")
-    code = _dtype_code(q)
-    n_pages, kv_heads, page, d = _check_cache(cache, q)
-    t, heads, dq = q.shape
-    if dq != d or kv_heads == 0 or heads % kv_heads:
-        raise ValueError(f"q is {tuple(q.shape)}, the cache has {kv_heads} heads of {d}")
-    batch, width = _table(block_table, q)
-    _ints(seq_lens, "seq_lens", (batch,), q)
-    cu = 0
-    if cu_seqlens is not None:
-        _ints(cu_seqlens, "cu_seqlens", (batch + 1,), q)
-        cu = cu_seqlens.data_ptr()
-    elif t != batch:
-        raise ValueError(f"{t} query tokens for {batch} sequences need cu_seqlens")
-    out = _out_like(out, q)
-    need = _lib.load().gq_attention_paged_workspace(t, batch, cu != 0, heads, kv_heads, d, page, width)
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    _launch("gq_attention_paged", q, _PAGED_ARGS.pack(
-        cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), n_pages, kv_heads, page, d, *_of(out), *_of(q), code, t,
-        heads, block_table.data_ptr(), width, seq_lens.data_ptr(), cu, batch, d ** -0.5 if scale is None else scale, ws.data_ptr() if need else 0, need))
-    return out
+    return _serving.attention_paged(q, *cache, block_table, seq_lens, cu_seqlens, scale, out)
 
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, ignore_index: int = -100) -> TokenLogprobs:
@@ -820,29 +658,4 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, ign
     entropy and its ``top`` (0..32) most likely words, ties to the lowest index; everything in fp32 from one read of the
     logits.  Logits of any row stride are taken as they are (a slice of sequences without their last token is copied).
     A token equal to ``ignore_index`` gives 0, any other that is no word NaN; -inf is a word that cannot come."""
-    _no_grad(logits)
-    if not isinstance(logits, torch.Tensor) or not isinstance(tokens, torch.Tensor):
-        raise TypeError("logits and tokens: expected tensors")
-    if not logits.is_cuda:
-        raise ValueError(f"logits: must live on the GPU (got {logits.device}); there is no CPU path")
-    code = 2 if logits.dtype is torch.float32 else _dtype_code(logits)
-    shape = tokens.shape
-    if logits.dim() == 0 or shape != logits.shape[:-1] or tokens.dtype is not torch.int64 or tokens.get_device() != logits.get_device():
-        raise ValueError(f"logits are {tuple(logits.shape)} on {logits.device}, tokens {tokens.dtype} {tuple(tokens.shape)} on {tokens.device}")
-    vocab = logits.shape[-1]
-    if vocab == 0 or not 0 <= top <= vocab:
-        raise ValueError(f"{top} alternatives of {vocab} words")
-    rows = logits if logits.dim() == 2 else logits.reshape(-1, vocab)
-    n = tokens.numel()
-    stride = rows.stride(0) if n > 1 else vocab
-    if n and (vocab > 1 and rows.stride(1) != 1 or stride < vocab):
-        rows, stride = rows.contiguous(), vocab
-    if not tokens.is_contiguous():
-        tokens = tokens.contiguous()
-    lp, ent = torch.empty((2, *shape), dtype=torch.float32, device=logits.device).unbind(0)
-    tlp = tok = None
-    if top:
-        tlp, tok = lp.new_empty((*shape, top)), torch.empty((*shape, top), dtype=torch.int64, device=logits.device)
-    _launch("gq_token_logprobs", logits, _LOGPROBS_ARGS.pack(rows.data_ptr(), code, n, stride, vocab, tokens.data_ptr(), ignore_index, lp.data_ptr(),
-                                                             ent.data_ptr(), top, tlp.data_ptr() if top else 0, tok.data_ptr() if top else 0))
-    return TokenLogprobs(lp, ent, tlp, tok)
+    return TokenLogprobs(*_serving.token_logprobs(logits, tokens, top, ignore_index))
