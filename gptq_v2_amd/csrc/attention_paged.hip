@@ -321,9 +321,10 @@ __global__ __launch_bounds__(256, NQ == 4 ? 1 : 2) void attention_paged_kernel(c
                     s[nt][i][j] = y;
                     top = fmaxf(top, y);
                 }
-            top = fmaxf(top, __shfl_xor(top, 16, 64));
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
-            if (__any(top > mx[nt])) {
+            top = gq_max_xor32(gq_max_xor16(top));
+            // M follows the maximum only when that is more than 2^8 above it: weights up to 256 instead of 1, and O is
+            // rescaled in a wave's first tile instead of in most (some row of 16 finds a new maximum in nearly every one)
+            if (__any(top > mx[nt] + 8.f)) {
                 const float to = fmaxf(top, mx[nt]);
                 const float f = mx[nt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx[nt] - to);
                 mx[nt] = to;

@@ -175,7 +175,7 @@ __global__ __launch_bounds__(256, 2) void attention_prompt_kernel(const PromptAr
         for (int tb = 0; tb < 2; ++tb)
 #pragma unroll
             for (int r = 0; r < 16; ++r) top = fmaxf(top, s[tb][r]);
-        top = fmaxf(top, __shfl_xor(top, 32, 64)) * a.scale;
+        top = gq_max_xor32(top) * a.scale;
         // The weights are 2^(s - mx) for an mx that follows the row's maximum only when that is more than 8 above it: up to
         // 256 instead of 1, which costs them no precision, and O is rescaled once or twice a row instead of in most tiles
         // (one of the wave's 32 rows finds a new maximum in nearly every tile; 4 x 2048 tokens 189 -> 180 us).

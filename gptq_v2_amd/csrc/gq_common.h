@@ -48,6 +48,19 @@ typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 static inline int64_t gq_cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 static inline int64_t gq_round_up(int64_t a, int64_t b) { return gq_cdiv(a, b) * b; }
 
+// The larger of x here and in the lane 32 (16) away: a swap of half waves (of every second row of 16 lanes) by the vector
+// unit, without the way through LDS that a shuffle takes.
+__device__ __forceinline__ float gq_max_xor32(float x)
+{
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float gq_max_xor16(float x)
+{
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
 __device__ __forceinline__ float gq_bf16_to_f32(unsigned short b)
 {
     return __uint_as_float(((unsigned int)b) << 16);
