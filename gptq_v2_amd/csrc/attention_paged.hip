@@ -177,7 +177,7 @@ __global__ __launch_bounds__(256, NQ == 4 ? 1 : 2) void attention_paged_kernel(c
     __syncthreads();
 
     // The pages of a tile, in scalar registers; the entries of the table are fetched a tile before they are used.
-    bool bad = false;   // a token that should be there lies on no page
+    bool bad = runs > a.n_splits;   // a token that should be there lies on no page (the table ends within the runs)
     const int32_t *table = a.table + (int64_t)it.b * a.table_width;
     struct Pages {
         int id[NP];
@@ -309,7 +309,7 @@ __global__ __launch_bounds__(256, NQ == 4 ? 1 : 2) void attention_paged_kernel(c
             copy_k(t + 4, now);
             load_scales(now);
         }
-        vs = fmaxf(vs, 1e-30f);   // a scale of 0 must not become an infinite weight
+        vs = fmaxf(vs, 0x1p-100f);   // a scale of 0 must not become an infinite weight
         const float mul = a.scale * ks, add = __builtin_amdgcn_logf(vs), inv = 1.f / vs;
         f16x8 p[NQ][2];
 #pragma unroll
@@ -620,17 +620,18 @@ extern "C" int gq_attention_paged(const gq_attention_paged_args *args, gq_stream
                (long long)n_heads, (long long)n_kv_heads, (long long)head_dim, (long long)page);
     GQ_REQUIRE(cu_seqlens || n_tokens == batch, "gq_attention_paged: %lld tokens for %lld sequences need cu_seqlens", (long long)n_tokens,
                (long long)batch);
-    GQ_REQUIRE(softmax_scale > 0.f && softmax_scale < INFINITY, "gq_attention_paged: the softmax scale must be positive and finite");
+    GQ_REQUIRE(softmax_scale > 0.f && softmax_scale * PA_LOG2E < INFINITY, "gq_attention_paged: the softmax scale must be positive and finite");
     if (n_tokens == 0 || batch == 0) return GQ_OK;
     GQ_REQUIRE(out.data && q.data && seq_lens && (table_width == 0 || block_table) && cache.k_codes && cache.v_codes && cache.k_scale && cache.v_scale,
                "gq_attention_paged: NULL pointer");
     GQ_REQUIRE(q.token_stride % 8 == 0 && q.head_stride % 8 == 0 && out.token_stride % 8 == 0 && out.head_stride % 8 == 0,
                "gq_attention_paged: strides must be multiples of 8 elements");
+    GQ_REQUIRE(gq_rows_apart(out, n_tokens, n_heads, head_dim), "gq_attention_paged: rows of out overlap");
     GQ_REQUIRE((((uintptr_t)out.data | (uintptr_t)q.data | (uintptr_t)cache.k_codes | (uintptr_t)cache.v_codes | (uintptr_t)workspace) & 15) == 0,
                "gq_attention_paged: pointers must be 16-byte aligned");
     const Plan p = paged_plan(n_tokens, batch, cu_seqlens != nullptr, n_heads, n_kv_heads, page, table_width);
     GQ_REQUIRE(n_pages > 0, "gq_attention_paged: a cache without pages");
-    GQ_REQUIRE(n_pages < ((int64_t)1 << 31) && p.n_items * n_kv_heads < ((int64_t)1 << 31) && n_tokens * n_heads < ((int64_t)1 << 31), "gq_attention_paged: too many query rows for one call");
+    GQ_REQUIRE(n_pages < ((int64_t)1 << 31) && p.n_items * n_kv_heads < GQ_MAX_THREADS / 256 && n_tokens * n_heads < ((int64_t)1 << 31), "gq_attention_paged: too many query rows for one call");
     const size_t need = p.n_splits == 1 ? 0 : (size_t)n_tokens * n_heads * p.n_splits * (head_dim + 4) * sizeof(float);
     if (workspace_bytes < need || (need && !workspace)) {
         gq_set_error("gq_attention_paged: workspace of %zu bytes, %zu needed", workspace_bytes, need);

@@ -333,18 +333,19 @@ extern "C" int gq_attention_prompt(const gq_attention_prompt_args *args, gq_stre
                (long long)n_heads, (long long)n_kv_heads);
     GQ_REQUIRE(n_tokens >= 0 && n_tokens < ((int64_t)1 << 30) && batch >= 0 && batch < (1 << 24), "gq_attention_prompt: bad number of tokens or sequences");
     GQ_REQUIRE(cu_seqlens || batch == 1 || n_tokens == 0, "gq_attention_prompt: %lld sequences need cu_seqlens", (long long)batch);
-    GQ_REQUIRE(softmax_scale > 0.f && softmax_scale < INFINITY, "gq_attention_prompt: the softmax scale must be positive and finite");
+    GQ_REQUIRE(softmax_scale > 0.f && softmax_scale * AP_LOG2E < INFINITY, "gq_attention_prompt: the softmax scale must be positive and finite");
     if (n_tokens == 0 || batch == 0) return GQ_OK;
     GQ_REQUIRE(out.data && q.data && k.data && v.data, "gq_attention_prompt: NULL pointer");
     GQ_REQUIRE(out.token_stride % 8 == 0 && out.head_stride % 8 == 0 && q.token_stride % 8 == 0 && q.head_stride % 8 == 0 && k.token_stride % 8 == 0 &&
                    k.head_stride % 8 == 0 && v.token_stride % 8 == 0 && v.head_stride % 8 == 0,
                "gq_attention_prompt: strides must be multiples of 8 elements");
+    GQ_REQUIRE(gq_rows_apart(out, n_tokens, n_heads, head_dim), "gq_attention_prompt: rows of out overlap");
     // a tile of 64 rows is addressed by 32-bit offsets, and a row must lie behind the one before it
     GQ_REQUIRE(n_tokens == 1 || (k.token_stride >= head_dim && v.token_stride >= head_dim && k.token_stride <= (1 << 23) && v.token_stride <= (1 << 23)),
                "gq_attention_prompt: token strides of k and v must be in head_dim..2^23");
     GQ_REQUIRE((((uintptr_t)out.data | (uintptr_t)q.data | (uintptr_t)k.data | (uintptr_t)v.data) & 15) == 0, "gq_attention_prompt: pointers must be 16-byte aligned");
     const int64_t n_items = cu_seqlens ? n_tokens / AP_Q + batch : gq_cdiv(n_tokens, AP_Q);
-    GQ_REQUIRE(n_items * n_heads < ((int64_t)1 << 31), "gq_attention_prompt: too many tokens for one call");
+    GQ_REQUIRE(n_items * n_heads < GQ_MAX_THREADS / 256, "gq_attention_prompt: too many tokens for one call");
     PromptArgs a;
     a.q = q.data, a.k = k.data, a.v = v.data, a.out = out.data;
     a.q_tok = q.token_stride, a.q_head = q.head_stride, a.k_tok = k.token_stride, a.k_head = k.head_stride;

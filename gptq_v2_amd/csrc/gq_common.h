@@ -48,6 +48,18 @@ typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 static inline int64_t gq_cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 static inline int64_t gq_round_up(int64_t a, int64_t b) { return gq_cdiv(a, b) * b; }
 
+// threads that one dimension of a launch can count
+constexpr int64_t GQ_MAX_THREADS = (int64_t)1 << 32;
+
+// No two rows of an output lie on each other: heads within a token's stride, or tokens within a head's.
+static inline bool gq_rows_apart(const gq_rows &x, int64_t n_tokens, int64_t n_heads, int64_t head_dim)
+{
+    const int64_t most = (int64_t)1 << 62, t = n_tokens > 1 ? x.token_stride : most, h = n_heads > 1 ? x.head_stride : most;
+    if (t < head_dim || h < head_dim) return false;
+    if (n_tokens == 1 || n_heads == 1) return true;
+    return t > most / n_tokens || h > most / n_heads || t >= (n_heads - 1) * h + head_dim || h >= (n_tokens - 1) * t + head_dim;
+}
+
 // The larger of x here and in the lane 32 (16) away: a swap of half waves (of every second row of 16 lanes) by the vector
 // unit, without the way through LDS that a shuffle takes.
 __device__ __forceinline__ float gq_max_xor32(float x)

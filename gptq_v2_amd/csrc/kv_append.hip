@@ -390,6 +390,7 @@ extern "C" int gq_kv_append(const gq_kv_append_args *args, gq_stream_t stream)
     GQ_REQUIRE(k.token_stride % 8 == 0 && k.head_stride % 8 == 0 && v.token_stride % 8 == 0 && v.head_stride % 8 == 0 &&
                    (!q.data || (q.token_stride % 8 == 0 && q.head_stride % 8 == 0 && q_out.token_stride % 8 == 0 && q_out.head_stride % 8 == 0)),
                "gq_kv_append: strides must be multiples of 8 elements");
+    GQ_REQUIRE(!q.data || gq_rows_apart(q_out, n_tokens, n_heads, head_dim), "gq_kv_append: rows of q_out overlap");
     GQ_REQUIRE((((uintptr_t)cache.k_codes | (uintptr_t)cache.v_codes | (uintptr_t)k.data | (uintptr_t)v.data | (uintptr_t)q.data | (uintptr_t)q_out.data | (uintptr_t)cos_t |
                  (uintptr_t)sin_t) & 15) == 0, "gq_kv_append: pointers must be 16-byte aligned");
     AppendArgs a;
@@ -410,7 +411,7 @@ extern "C" int gq_kv_append(const gq_kv_append_args *args, gq_stream_t stream)
     const int64_t q_blocks = q.data ? n_tokens * a.q_parts : 0;
     const size_t lds = cu_seqlens ? (size_t)(page * head_dim) : 0;
     const int64_t grid = n_items * n_kv_heads * 2 + q_blocks;
-    GQ_REQUIRE(grid < ((int64_t)1 << 31), "gq_kv_append: too many tokens for one call");
+    GQ_REQUIRE(grid < GQ_MAX_THREADS / threads, "gq_kv_append: too many tokens for one call");
     a.n_items = (int)n_items;
     if (dtype == GQ_F16) hipLaunchKernelGGL(kv_append_kernel<_Float16>, dim3((unsigned)grid), dim3(threads), lds, (hipStream_t)stream, a);
     else hipLaunchKernelGGL(kv_append_kernel<__bf16>, dim3((unsigned)grid), dim3(threads), lds, (hipStream_t)stream, a);

@@ -63,7 +63,7 @@ struct Stat {
     __device__ __forceinline__ void move(float to)
     {
         const float d = m - to, f = __builtin_amdgcn_exp2f(d);
-        t = s == 0.f ? 0.f : fmaf(d, s, t) * f;
+        t = f == 0.f ? 0.f : fmaf(d, s, t) * f;   // (d s may overflow where f is 0)
         s *= f;
         m = to;
     }
@@ -210,10 +210,10 @@ __global__ __launch_bounds__(NT) void token_logprobs_kernel(const T *__restrict_
     __syncthreads();
     st.s = lp_sum<WAVES>(sm_s[lane % WAVES]);
     st.t = lp_sum<WAVES>(sm_t[lane % WAVES]);
-    // No sum: a row of numbers beyond the reference's range, of -inf alone, with NaN or +inf.  It is taken again, from its
-    // maximum; the last three come out as NaN.
+    // No sum: a row of numbers so large that their reference's own rounding (2^-24 of it) over- or underflows 2^y, of -inf
+    // alone, with NaN or +inf.  It is taken again, from its maximum; the last three come out as NaN.
     float log_s = log2f(st.s), unit = LP_LN2, m = st.m;
-    const bool odd = !(st.s > 0.f && st.s < INFINITY);
+    const bool odd = !(st.s > 0.f && st.s < INFINITY && fabsf(st.t) < INFINITY);
     if (odd) {
         __syncthreads();
         float most = -INFINITY;
@@ -240,7 +240,11 @@ __global__ __launch_bounds__(NT) void token_logprobs_kernel(const T *__restrict_
         log_s = st.s > 0.f ? logf(st.s) : NAN;
         unit = 1.f;
     }
-    const auto log_p = [&](float v) { return ((odd ? v - m : fmaf(v, LP_LOG2E, -m)) - log_s) * unit; };
+    const auto log_p = [&](float v) {
+        const float y = odd ? v - m : fmaf(v, LP_LOG2E, -m);
+        // (a number near the type's lowest is out of range in units of log 2)
+        return y == -INFINITY ? v - (m + log_s) * unit : (y - log_s) * unit;
+    };
     if (tid == 0) {
         float lp = NAN;
         if (token == ignore_index) lp = 0.f;
@@ -343,7 +347,7 @@ extern "C" int gq_token_logprobs(const gq_token_logprobs_args *args, gq_stream_t
     int64_t *top_token = args->top_token;
     GQ_REQUIRE(dtype == GQ_F16 || dtype == GQ_BF16 || dtype == GQ_F32, "gq_token_logprobs: dtype %lld is none of fp16 (0), bf16 (1), fp32 (2)",
                (long long)dtype);
-    GQ_REQUIRE(n_rows >= 0 && n_rows < ((int64_t)1 << 31), "gq_token_logprobs: bad row count %lld", (long long)n_rows);
+    GQ_REQUIRE(n_rows >= 0 && n_rows < GQ_MAX_THREADS / 256, "gq_token_logprobs: bad row count %lld", (long long)n_rows);
     GQ_REQUIRE(vocab > 0 && vocab <= (1 << 30), "gq_token_logprobs: vocab must be in 1..2^30");
     GQ_REQUIRE(args->top >= 0 && args->top <= LP_MAX_TOP && args->top <= vocab, "gq_token_logprobs: %lld alternatives: 0..%d of the vocabulary can be asked for",
                (long long)args->top, LP_MAX_TOP);

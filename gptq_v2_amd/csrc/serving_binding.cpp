@@ -114,10 +114,11 @@ const int32_t *table(const at::Tensor &t, const at::Tensor &like)
     return (const int32_t *)t.data_ptr();
 }
 
+// (a dimension of size 1 has any stride)
 gq_rows rows_of(const at::Tensor &t)
 {
     if (!t.defined()) return {nullptr, 0, 0};
-    return {t.data_ptr(), t.stride(0), t.stride(1)};
+    return {t.data_ptr(), t.size(0) > 1 ? t.stride(0) : 0, t.size(1) > 1 ? t.stride(1) : 0};
 }
 
 at::Tensor out_like(PyObject *o, const char *name, const at::Tensor &q)

@@ -407,7 +407,8 @@ int gq_rope_inplace(void *x, int64_t row_stride, const void *cos_t, const void *
  * Sequences are packed: row i of a [n_tokens][heads][head_dim] tensor belongs to the sequence b with
  * cu_seqlens[b] <= i < cu_seqlens[b + 1] (int32, batch + 1 of them, rising).  Rows behind cu_seqlens[batch] are neither
  * read nor written.  Such tensors are given by a token and a head stride in elements (multiples of 8, 16-byte aligned
- * pointers), so that q, k and v may be slices of one merged product.  Query head h reads kv head h / (n_heads / n_kv_heads).
+ * pointers), so that q, k and v may be slices of one merged product.  Outputs overlap neither themselves nor what is read,
+ * where nothing else is said.  Query head h reads kv head h / (n_heads / n_kv_heads).
  * The arguments of a call stand in a struct of 8-byte fields, read during the call only.
  */
 typedef struct gq_rows {

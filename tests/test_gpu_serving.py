@@ -359,6 +359,31 @@ def test_paged_attention_of_a_bad_table(amd, gpu):
     _close(got[1:2], want, bound)
 
 
+@pytest.mark.parametrize("page,width", [(16, 16), (64, 4), (32, 9), (128, 16), (16, 512)])
+@pytest.mark.parametrize("more", [1, 40, 70000])
+def test_paged_attention_of_sequences_longer_than_their_table(amd, gpu, page, width, more):
+    """NaN, also where the table ends with a tile or with the last run of one; a full table is none."""
+    full = page * width
+    c, dev, table = _filled(amd, gpu, [full, full], 1, page, 64, seed=9)
+    q = torch.randn(2, 4, 64, generator=_gen(6)).half()
+    lens = torch.tensor([full, full + more], dtype=torch.int32)
+    got = amd.ops.attention_paged(q.to(gpu), dev, table.to(gpu), lens.to(gpu)).cpu()
+    assert torch.isnan(got[1]).all()
+    _check_paged(got[:1], q[:1], c, table[:1], [full], [1], torch.float16)
+
+
+def test_paged_attention_of_the_smallest_scales(amd, gpu):
+    """Values of 2^-100 times a code: bf16 holds the result."""
+    c, dev, table = _filled(amd, gpu, [50, 200], 1, 16, 64, seed=10)
+    q = torch.randn(2, 4, 64, generator=_gen(7)).bfloat16()
+    lens = torch.tensor([50, 200], dtype=torch.int32, device=gpu)
+    one = dev._replace(v_scale=torch.ones_like(dev.v_scale))
+    low = dev._replace(v_scale=torch.full_like(dev.v_scale, 2.0 ** -100))
+    a, b = (amd.ops.attention_paged(q.to(gpu), x, table.to(gpu), lens).double() for x in (one, low))
+    # the weights differ by the rounding of y + log2 vs alone: |y| < 128 rounds by 2^-18, the weight by ln 2 of that
+    assert ((b * 2.0 ** 100 - a).abs() <= 2.0 ** -7 * a.abs() + 2.0 ** -9).all()
+
+
 def test_paged_attention_keeps_later_nan_from_earlier_rows(amd, gpu):
     """A NaN among the values (keys) of the second of three query tokens does not reach the first."""
     for part in ("k", "v"):
@@ -465,6 +490,38 @@ def test_token_logprobs_infinities_and_nan(amd, gpu):
     for dtype in (torch.float32, torch.float16):
         y = x.to(dtype)
         _check_logprobs(amd.ops.token_logprobs(y.to(gpu), tokens.to(gpu), top=12), y, tokens, 12)
+
+
+@pytest.mark.parametrize("rows,vocab", [(3, 32003), (600, 1003), (2, 40)])
+def test_token_logprobs_of_masked_words(amd, gpu, rows, vocab):
+    """Words masked by the type's lowest value: all of a row (a uniform one), all but a few, whole stretches; the same by -inf
+    but for the row without a word."""
+    gen = _gen(vocab)
+    for dtype in (torch.float16, torch.bfloat16, torch.float32):
+        for low in (torch.finfo(dtype).min, -math.inf, *((-1e30, -1e38, -2e38) if dtype != torch.float16 else (-1e4,))):
+            x = (3 * torch.randn(rows, vocab, generator=gen)).to(dtype)
+            x[0, :] = low
+            x[0, 17], x[0, vocab - 1] = 1.5, 1.0
+            if low > -math.inf:
+                x[1, :] = low
+            else:
+                x[1, : vocab // 2] = low
+            if rows > 2:
+                x[2, 8:vocab - 8] = low
+            tokens = torch.randint(0, vocab, (rows,), generator=gen)
+            tokens[0] = 17
+            _check_logprobs(amd.ops.token_logprobs(x.to(gpu), tokens.to(gpu), top=6), x, tokens, 6)
+
+
+def test_token_logprobs_of_large_numbers(amd, gpu):
+    """Logits far from 0, where their differences are exact but their size is not small; the type's largest and lowest."""
+    gen = _gen(12)
+    for dtype, base in (*((torch.float32, 2.0 ** 31 + 2.0 ** 20 * i) for i in range(12)), (torch.float32, 2.0 ** 20), (torch.float32, -2.0 ** 22), (torch.float32, 2.0 ** 100), (torch.float32, -3.0e38), (torch.bfloat16, 3.0e38), (torch.float16, 6.0e4)):
+        x = torch.randint(-8, 9, (4, 5003), generator=gen).to(torch.float64)
+        x = (base + x * max(1.0, abs(base) * torch.finfo(dtype).eps)).clamp(torch.finfo(dtype).min, torch.finfo(dtype).max).to(dtype)
+        tokens = torch.randint(0, 5003, (4,), generator=gen)
+        tokens[0] = int(x[0].argmax())
+        _check_logprobs(amd.ops.token_logprobs(x.to(gpu), tokens.to(gpu), top=4), x, tokens, 4)
 
 
 def test_token_logprobs_tokens_shapes_and_strides(amd, gpu):
@@ -644,7 +701,7 @@ def test_serving_operators_refuse_what_they_do_not_take(amd, gpu):
         lambda: ops.attention_prompt(q, k.bfloat16(), k), lambda: ops.attention_prompt(torch.zeros(4, 4, 65, **h)[..., :64], k, k),
         lambda: ops.attention_prompt(q.transpose(1, 2).contiguous().transpose(1, 2), k, k), lambda: ops.attention_prompt(q, k.expand(4, 2, 64)[:1].expand(4, 2, 64), k),
         lambda: ops.attention_prompt(torch.zeros(4, 4, 136, **h), torch.zeros(4, 2, 136, **h), torch.zeros(4, 2, 136, **h)),
-        lambda: ops.attention_prompt(q, k, k, out=q[:3]), lambda: ops.attention_prompt(q.cpu(), k, k),
+        lambda: ops.attention_prompt(q, k, k, out=q[:3]), lambda: ops.attention_prompt(q, k, k, out=torch.zeros(1, 4, 64, **h).expand(4, 4, 64)), lambda: ops.attention_prompt(q.cpu(), k, k),
     ]
     cache = ops.PagedCache.empty(4, 2, 16, 64, gpu)
     table = torch.zeros(4, 2, dtype=torch.int32, device=gpu)
