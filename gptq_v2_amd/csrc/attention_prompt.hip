@@ -64,7 +64,9 @@ __global__ __launch_bounds__(256, 2) void attention_prompt_kernel(const PromptAr
     constexpr int NCH = DP / 8;                       // 16-byte chunks of a row
     constexpr int PIECES = AP_K * NCH / 256;          // copy instructions per wave and tile
     constexpr int STEPS = DP / 16, DT = DP / 32;
-    __shared__ __attribute__((aligned(1024))) T sm_k[2][AP_K * DP], sm_v[2][AP_K * DP];
+    // Four objects, so that the compiler's own waits tell the copies into one from those into the next: of one object it
+    // makes the reads of a tile wait for the copies of the tile after it.
+    __shared__ __attribute__((aligned(1024))) T sm_k0[AP_K * DP], sm_k1[AP_K * DP], sm_v0[AP_K * DP], sm_v1[AP_K * DP];
 
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);   // uniform, so that what follows from it is scalar
@@ -113,19 +115,24 @@ __global__ __launch_bounds__(256, 2) void attention_prompt_kernel(const PromptAr
         v_off[j] = 8 * c < d ? r * v_row + 16 * c : AP_OUT_OF_RANGE;
     }
     const T *kb = (const T *)a.k + row0 * a.k_tok + head_kv * a.k_head, *vb = (const T *)a.v + row0 * a.v_tok + head_kv * a.v_head;
-    const auto stage = [&](int j, int buf) {
+    const auto stage = [&](int j, T *to_k, T *to_v) {
         const int rows = len - j * AP_K < AP_K ? len - j * AP_K : AP_K;
         const ap_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((void *)(kb + (int64_t)j * AP_K * a.k_tok), 0, (int)((rows - 1) * k_row + 2 * d), 0x00020000);
         const ap_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((void *)(vb + (int64_t)j * AP_K * a.v_tok), 0, (int)((rows - 1) * v_row + 2 * d), 0x00020000);
 #pragma unroll
         for (int p = 0; p < PIECES; ++p)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, GQ_LDS_PTR(void, &sm_k[buf][(wave * 64 + 256 * p) * 8]), 16, (int)k_off[p], 0, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, GQ_LDS_PTR(void, to_k + (wave * 64 + 256 * p) * 8), 16, (int)k_off[p], 0, 0, 0);
 #pragma unroll
         for (int p = 0; p < PIECES; ++p)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, GQ_LDS_PTR(void, &sm_v[buf][(wave * 64 + 256 * p) * 8]), 16, (int)v_off[p], 0, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, GQ_LDS_PTR(void, to_v + (wave * 64 + 256 * p) * 8), 16, (int)v_off[p], 0, 0, 0);
+    };
+    // all copies under way have arrived, everybody's (a barrier alone does not wait for the copies)
+    const auto arrived = [] {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
     };
 
-    stage(0, 0);
+    stage(0, sm_k0, sm_v0);
     vec qf[STEPS];
     {
         const T *qp = (const T *)a.q + (row0 + (row < len ? row : 0)) * a.q_tok + head * a.q_head;
@@ -151,6 +158,9 @@ __global__ __launch_bounds__(256, 2) void attention_prompt_kernel(const PromptAr
     const int see = a.causal ? (row < len - 1 ? row : len - 1) : len - 1;   // the last key this row sees
 
     const auto compute = [&](auto masked, int j, const T *tk, const T *tv) {
+        int lane = tid & 63;
+        if constexpr (masked) asm volatile("" : "+v"(lane));   // (for a few tiles no addresses are kept in registers)
+        const int col = lane & 31, h = lane >> 5;
         f32x16 s[2];
 #pragma unroll
         for (int tb = 0; tb < 2; ++tb) {
@@ -260,21 +270,21 @@ __global__ __launch_bounds__(256, 2) void attention_prompt_kernel(const PromptAr
     const int n_clear = (a.causal ? (q0 + 1) / AP_K : len / AP_K) & ~1;
     int j = 0;
     for (; j < n_clear; j += 2) {
-        __syncthreads();
-        stage(j + 1, 1);
-        compute(std::false_type(), j, sm_k[0], sm_v[0]);
-        __syncthreads();
-        if (j + 2 < n_tiles) stage(j + 2, 0);
-        compute(std::false_type(), j + 1, sm_k[1], sm_v[1]);
+        arrived();
+        stage(j + 1, sm_k1, sm_v1);
+        compute(std::false_type(), j, sm_k0, sm_v0);
+        arrived();
+        if (j + 2 < n_tiles) stage(j + 2, sm_k0, sm_v0);
+        compute(std::false_type(), j + 1, sm_k1, sm_v1);
     }
     for (; j < n_tiles; j += 2) {
-        __syncthreads();
-        if (j + 1 < n_tiles) stage(j + 1, 1);
-        if (j < my_tiles) compute(std::true_type(), j, sm_k[0], sm_v[0]);
+        arrived();
+        if (j + 1 < n_tiles) stage(j + 1, sm_k1, sm_v1);
+        if (j < my_tiles) compute(std::true_type(), j, sm_k0, sm_v0);
         if (j + 1 >= n_tiles) break;
-        __syncthreads();
-        if (j + 2 < n_tiles) stage(j + 2, 0);
-        if (j + 1 < my_tiles) compute(std::true_type(), j + 1, sm_k[1], sm_v[1]);
+        arrived();
+        if (j + 2 < n_tiles) stage(j + 2, sm_k0, sm_v0);
+        if (j + 1 < my_tiles) compute(std::true_type(), j + 1, sm_k1, sm_v1);
     }
 
     l += __shfl_xor(l, 32, 64);
@@ -282,7 +292,7 @@ __global__ __launch_bounds__(256, 2) void attention_prompt_kernel(const PromptAr
     // A lane holds 4 adjacent channels here and there of its row: through LDS (the wave's 32 rows, places as in the tiles),
     // so that rows are written in whole lines.
     __syncthreads();
-    T *so = &sm_k[0][0] + wave * 32 * DP;
+    T *so = sm_k0 + wave * 32 * DP;
 #pragma unroll
     for (int t = 0; t < DT; ++t)
 #pragma unroll
@@ -350,6 +360,7 @@ extern "C" int gq_attention_prompt(const gq_attention_prompt_args *args, gq_stre
     a.q = q.data, a.k = k.data, a.v = v.data, a.out = out.data;
     a.q_tok = q.token_stride, a.q_head = q.head_stride, a.k_tok = k.token_stride, a.k_head = k.head_stride;
     a.v_tok = v.token_stride, a.v_head = v.head_stride, a.o_tok = out.token_stride, a.o_head = out.head_stride;
+    if (n_tokens == 1) a.k_tok = a.v_tok = head_dim;   // (any stride may stand there)
     a.cu = cu_seqlens, a.n_tokens = n_tokens, a.batch = (int)batch, a.n_heads = (int)n_heads, a.group = (int)(n_heads / n_kv_heads);
     a.head_dim = (int)head_dim, a.n_items = (int)n_items, a.causal = args->causal != 0, a.scale = softmax_scale * AP_LOG2E;
     return dtype == GQ_F16 ? launch_prompt<_Float16>(a, (hipStream_t)stream) : launch_prompt<__bf16>(a, (hipStream_t)stream);
