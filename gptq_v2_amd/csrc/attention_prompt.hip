@@ -152,33 +152,40 @@ __global__ __launch_bounds__(256, 2) void attention_prompt_kernel(const PromptAr
     float mx = -INFINITY, l = 0.f;
     const int q_last = q0 + AP_Q - 1 < len - 1 ? q0 + AP_Q - 1 : len - 1;
     const int n_tiles = ((a.causal ? q_last : len - 1) + AP_K) / AP_K;
-    // tiles that some row of this wave sees
-    const int my_last = q0 + wave * 32 + 31 < len - 1 ? q0 + wave * 32 + 31 : len - 1;
-    const int my_tiles = a.causal ? (my_last + AP_K) / AP_K : n_tiles;
-    const int see = a.causal ? (row < len - 1 ? row : len - 1) : len - 1;   // the last key this row sees
+    // This wave's rows all see the first my_clear tiles, and of the tile after them the first `blocks` blocks of 32 tokens,
+    // the last of those only in part.  (Tiles and waves begin at multiples of 32: the diagonal passes through one block.
+    // Tokens behind the sequence are behind all its rows.)
+    const int first_row = q0 + wave * 32;
+    const int my_clear = first_row < len ? (a.causal ? first_row + 1 : len) / AP_K : 0;
+    const int blocks = first_row < len ? ((a.causal ? first_row + 32 : len) - my_clear * AP_K + 31) / 32 : 0;
+    const int see = a.causal ? row : len - 1;   // the last key this row sees
 
-    const auto compute = [&](auto masked, int j, const T *tk, const T *tv) {
+    // `tail`: of the tile only the first `blocks` (1 or 2) blocks of 32 tokens are visible, the last of them not to every
+    // row unless the tile is clear to this wave.
+    const auto compute = [&](auto tail, int j, const T *tk, const T *tv) {
         int lane = tid & 63;
-        if constexpr (masked) asm volatile("" : "+v"(lane));   // (for a few tiles no addresses are kept in registers)
+        if constexpr (tail) asm volatile("" : "+v"(lane));   // (for a few tiles no addresses are kept in registers)
         const int col = lane & 31, h = lane >> 5;
+        const int n_blocks = !tail || j < my_clear ? 2 : blocks, cut = !tail || j < my_clear ? 2 : blocks - 1;
         f32x16 s[2];
 #pragma unroll
         for (int tb = 0; tb < 2; ++tb) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[tb][r] = 0.f;
-            const int kr = 32 * tb + col, sw = ap_swizzle<DP>(kr);
+            if (tb < n_blocks) {
+                const int kr = 32 * tb + col, sw = ap_swizzle<DP>(kr);
 #pragma unroll
-            for (int st = 0; st < STEPS; ++st) {
-                const vec kf = *reinterpret_cast<const vec *>(tk + kr * DP + ((2 * st + h) ^ sw) * 8);
-                s[tb] = Mma<T>::run(kf, qf[st], s[tb]);
+                for (int st = 0; st < STEPS; ++st) {
+                    const vec kf = *reinterpret_cast<const vec *>(tk + kr * DP + ((2 * st + h) ^ sw) * 8);
+                    s[tb] = Mma<T>::run(kf, qf[st], s[tb]);
+                }
             }
-        }
-        if (masked) {
-#pragma unroll
-            for (int tb = 0; tb < 2; ++tb)
+            if (tb >= cut) {
+                const int rel = tb > cut ? -1 : see - (j * AP_K + 32 * tb) - 4 * h;
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    if (j * AP_K + 32 * tb + 8 * (r >> 2) + 4 * h + (r & 3) > see) s[tb][r] = -INFINITY;
+                    if (8 * (r >> 2) + (r & 3) > rel) s[tb][r] = -INFINITY;
+            }
         }
         float top = s[0][0];
 #pragma unroll
@@ -221,53 +228,67 @@ __global__ __launch_bounds__(256, 2) void attention_prompt_kernel(const PromptAr
             }
             return vf;
         };
+        if constexpr (!tail) {
 #pragma unroll
-        for (int t = 0; t < DT; ++t) {
-            if constexpr (!masked) {
+            for (int t = 0; t < DT; ++t)
 #pragma unroll
                 for (int s2 = 0; s2 < 4; ++s2) o[t] = Mma<T>::run(read_v(t, s2), p[s2], o[t]);
-            } else {
-                // 0 * inf and 0 * NaN are NaN: an infinity or NaN among these values must not reach the rows before it.
-                // Adding one to an exponent field of all ones carries into the sign's place.
-                vec vf[4];
-                unsigned found = 0;
+        } else {
 #pragma unroll
-                for (int s2 = 0; s2 < 4; ++s2) {
-                    vf[s2] = read_v(t, s2);
-                    unsigned x[4];
-                    __builtin_memcpy(x, &vf[s2], 16);
+            for (int tb = 0; tb < 2; ++tb) {
+                if (tb >= n_blocks) break;
+                if (tb != cut) {
 #pragma unroll
-                    for (int w = 0; w < 4; ++w) found |= (x[w] & 0x7fff7fffu) + Mma<T>::EXPONENT_ONE;
-                }
-                if (!__any((found & 0x80008000u) != 0)) {
+                    for (int t = 0; t < DT; ++t)
 #pragma unroll
-                    for (int s2 = 0; s2 < 4; ++s2) o[t] = Mma<T>::run(vf[s2], p[s2], o[t]);
+                        for (int s2 = 2 * tb; s2 < 2 * tb + 2; ++s2) o[t] = Mma<T>::run(read_v(t, s2), p[s2], o[t]);
                     continue;
                 }
-                // one token at a time, added only to the rows that see it
+                // 0 * inf and 0 * NaN are NaN: an infinity or NaN among these values must not reach the rows before it.
+                // Adding one to an exponent field of all ones carries into the sign's place.
 #pragma unroll
-                for (int s2 = 0; s2 < 4; ++s2)
-#pragma unroll 1
-                    for (int tok = 0; tok < 16; ++tok) {
-                        vec one = vf[s2];
+                for (int t = 0; t < DT; ++t) {
+                    vec vf[2];
+                    unsigned found = 0;
 #pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            if (8 * (i >> 2) + 4 * h + (i & 3) != tok) one[i] = static_cast<T>(0.f);
-                        f32x16 x;
+                    for (int i = 0; i < 2; ++i) {
+                        vf[i] = read_v(t, 2 * tb + i);
+                        unsigned x[4];
+                        __builtin_memcpy(x, &vf[i], 16);
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) x[r] = 0.f;
-                        x = Mma<T>::run(one, p[s2], x);
-                        if (j * AP_K + 16 * s2 + tok <= see) {
-#pragma unroll
-                            for (int r = 0; r < 16; ++r) o[t][r] += x[r];
-                        }
+                        for (int w = 0; w < 4; ++w) found |= (x[w] & 0x7fff7fffu) + Mma<T>::EXPONENT_ONE;
                     }
+                    if (!__any((found & 0x80008000u) != 0)) {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) o[t] = Mma<T>::run(vf[i], p[2 * tb + i], o[t]);
+                        continue;
+                    }
+                    // one token at a time, added only to the rows that see it
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll 1
+                        for (int tok = 0; tok < 16; ++tok) {
+                            vec one = vf[i];
+#pragma unroll
+                            for (int e = 0; e < 8; ++e)
+                                if (8 * (e >> 2) + 4 * h + (e & 3) != tok) one[e] = static_cast<T>(0.f);
+                            f32x16 x;
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) x[r] = 0.f;
+                            x = Mma<T>::run(one, p[2 * tb + i], x);
+                            if (j * AP_K + 32 * tb + 16 * i + tok <= see) {
+#pragma unroll
+                                for (int r = 0; r < 16; ++r) o[t][r] += x[r];
+                            }
+                        }
+                }
             }
         }
     };
 
-    // pairs of tiles that are visible to the whole workgroup, then those that may be masked
+    // pairs of tiles that are visible to the whole workgroup, then those that may be cut, each wave as far as it sees
     const int n_clear = (a.causal ? (q0 + 1) / AP_K : len / AP_K) & ~1;
+    const int my_tiles = my_clear + (blocks > 0);
     int j = 0;
     for (; j < n_clear; j += 2) {
         arrived();
