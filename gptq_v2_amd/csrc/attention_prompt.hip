@@ -86,17 +86,21 @@ __global__ __launch_bounds__(256, 2) void attention_prompt_kernel(const PromptAr
     if (a.cu) {
         // Sequence b's tiles start at item cu[b] / 128 + b: room for all of them without the host knowing the lengths.
         // The starts rise, so b is one less than the number of starts up to this item; 64 are looked at at a time.
-        int lo = -1;
+        // (The two starts that count are nearly always among those in the lanes.)
+        int lo = -1, c = 0, mine = 0;
         for (int b0 = 0; b0 < a.batch; b0 += 64) {
-            const bool before = b0 + lane < a.batch && a.cu[b0 + lane] / AP_Q + b0 + lane <= item;
-            const int c = __popcll(__ballot(before));
+            const int at = b0 + lane < a.batch ? b0 + lane : a.batch;
+            mine = a.cu[at];
+            c = __popcll(__ballot(b0 + lane < a.batch && mine / AP_Q + at <= item));
             lo += c;
             if (c < 64) break;
         }
         if (lo < 0) return;
         lo = __builtin_amdgcn_readfirstlane(lo);
-        row0 = a.cu[lo];
-        n = (int64_t)a.cu[lo + 1] - row0;
+        c = __builtin_amdgcn_readfirstlane(c);
+        const bool here = c > 0 && c < 64;
+        row0 = here ? __builtin_amdgcn_readlane(mine, c - 1) : a.cu[lo];
+        n = (here ? __builtin_amdgcn_readlane(mine, c) : a.cu[lo + 1]) - row0;
         const int64_t t = item - (row0 / AP_Q + lo);
         if (row0 < 0 || n <= 0 || row0 + n > a.n_tokens || t < 0 || t * AP_Q >= n) return;
         tile = (int)t;
