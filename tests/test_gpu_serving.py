@@ -77,6 +77,51 @@ def test_prompt_attention_against_64_bits(amd, gpu, lens, hq, hkv, d, causal, dt
     _check_prompt(amd.ops, x, views, lens, hq, hkv, causal, dtype)
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("d,dtype", [(64, torch.float16), (128, torch.bfloat16), (96, torch.float16)])
+def test_prompt_attention_at_the_borders_of_blocks(amd, gpu, causal, d, dtype):
+    """Lengths around the 32, 64 and 128 rows and tokens that blocks, tiles and workgroups have; more than 64 sequences, the
+    empty ones among them."""
+    lens = [m + e for m in (32, 64, 96, 128, 160, 192, 256) for e in (-1, 0, 1)]
+    x, views = _qkv(_gen(d), sum(lens), 2, 1, d, dtype, "merged", gpu)
+    _check_prompt(amd.ops, x, views, lens, 2, 1, causal, dtype)
+    many = [(7 * i) % 5 * (40 if i % 29 == 3 else 1) for i in range(200)]
+    x, views = _qkv(_gen(d + 1), sum(many) + 3, 2, 1, d, dtype, "merged", gpu)
+    _check_prompt(amd.ops, x, views, many, 2, 1, causal, dtype)
+
+
+@pytest.mark.parametrize("at", [0, 1, 31, 32, 63, 64, 95, 96, 127, 128, 138])
+def test_prompt_attention_keeps_infinite_values_from_earlier_rows_everywhere(amd, gpu, at):
+    """An infinite value of any token of a tile reaches the rows from its own on; of a following sequence, none at all."""
+    x, _ = _qkv(_gen(50), 139 + 20, 2, 1, 64, torch.float16, "plain", gpu)
+    x[at, 3, 5], x[139:, 2:] = math.inf, math.nan
+    y = x.to(gpu)
+    for causal in (True, False):
+        out = amd.ops.attention_prompt(y[:, :2], y[:, 2:3], y[:, 3:], _cu([139], gpu), causal=causal)[:139].cpu()
+        clean = x[:139].clone()
+        clean[at, 3] = 0.5
+        s = clean.double()
+        want, bound = ref.attend(s[:, :2], s[:, 2:3], s[:, 3:], 0 if causal else None, 64 ** -0.5, torch.float16)
+        first = at if causal else 0
+        _close(out[:first], want[:first], bound[:first])
+        rest = [c for c in range(64) if c != 5]
+        s[at, 3] = x[at, 3].double()
+        s[at, 3, 5] = 0.5
+        want, bound = ref.attend(s[:, :2], s[:, 2:3], s[:, 3:], 0 if causal else None, 64 ** -0.5, torch.float16)
+        _close(out[..., rest], want[..., rest], bound[..., rest])
+        assert not torch.isfinite(out[first:, :, 5]).any()
+
+
+def test_prompt_attention_of_one_token_with_any_stride(amd, gpu):
+    """A dimension of one element may have any stride: one row of a transposed or odd-strided tensor is taken."""
+    x = torch.randn(1, 4, 64, generator=_gen(51)).half()
+    for stride in (0, 3, 1 << 30):
+        q, k, v = (t.to(gpu).as_strided((1, n, 64), (stride, 64, 1)) for t, n in ((x[:, :2], 2), (x[:, 2:3], 1), (x[:, 3:], 1)))
+        got = amd.ops.attention_prompt(q, k, v)
+        # one key: its value
+        assert torch.equal(got.cpu(), x[:, 3:].expand(1, 2, 64))
+
+
 def test_prompt_attention_one_sequence_scale_and_large_scores(amd, gpu):
     """No cu_seqlens; a scale of its own; scores in the hundreds, where the softmax is a choice of one key."""
     x, views = _qkv(_gen(3), 150, 4, 4, 64, torch.float16, "merged", gpu)
@@ -247,6 +292,13 @@ def test_append_skips_what_has_no_place(amd, gpu):
     assert torch.equal(got[:len(pos)][has], want[has]) and torch.isnan(got[:len(pos)][~has]).all() and (got[len(pos):] == 5.0).all()
 
 
+def test_append_of_many_sequences(amd, gpu):
+    """More sequences than one look at the starts sees, empty ones and pages that are begun among them."""
+    c = Both(amd, gpu, 150, 3, 1, 16, 32, seed=23)
+    for i in range(3):
+        c.append([(5 * b + 3 * i) % 7 if b % 13 else 13 for b in range(150)], torch.float16, 32, i == 1, q_heads=2)
+
+
 def test_append_rotates_q_in_place(amd, gpu):
     gen = _gen(11)
     for inter in (False, True):
@@ -382,6 +434,24 @@ def test_paged_attention_of_the_smallest_scales(amd, gpu):
     a, b = (amd.ops.attention_paged(q.to(gpu), x, table.to(gpu), lens).double() for x in (one, low))
     # the weights differ by the rounding of y + log2 vs alone: |y| < 128 rounds by 2^-18, the weight by ln 2 of that
     assert ((b * 2.0 ** 100 - a).abs() <= 2.0 ** -7 * a.abs() + 2.0 ** -9).all()
+
+
+def test_paged_attention_of_many_ragged_sequences(amd, gpu):
+    lens = [(37 * b) % 90 for b in range(150)]
+    new = [min(n, (11 * b) % 4) for b, n in enumerate(lens)]
+    c, dev, table = _filled(amd, gpu, lens, 1, 32, 64, seed=24)
+    q = torch.randn(sum(new), 4, 64, generator=_gen(52)).half()
+    got = amd.ops.attention_paged(q.to(gpu), dev, table.to(gpu), torch.tensor(lens, dtype=torch.int32, device=gpu), _cu(new, gpu))
+    _check_paged(got, q, c, table, lens, new, torch.float16)
+
+
+def test_paged_attention_of_shared_pages(amd, gpu):
+    """Sequences that begin with the same pages, and one that names a page twice."""
+    c, dev, table = _filled(amd, gpu, [128, 128, 128], 2, 64, 64, seed=25)
+    table[1, 0], table[2, 1] = table[0, 0], table[2, 0]
+    q = torch.randn(3, 4, 64, generator=_gen(53)).half()
+    got = amd.ops.attention_paged(q.to(gpu), dev, table.to(gpu), torch.full((3,), 128, dtype=torch.int32, device=gpu))
+    _check_paged(got, q, c, table, [128] * 3, [1] * 3, torch.float16)
 
 
 def test_paged_attention_keeps_later_nan_from_earlier_rows(amd, gpu):
@@ -673,6 +743,25 @@ def test_serving_operators_run_on_the_current_stream(amd, gpu):
     assert torch.equal(got, want) and b is not None
     again = ops.token_logprobs(qkv.view(130, -1), torch.zeros(130, dtype=torch.int64, device=gpu), top=2)
     assert torch.equal(lp.logprob, again.logprob) and torch.equal(lp.top_token, again.top_token)
+
+
+def test_two_calls_at_once(amd, gpu):
+    """The same long sequence read from two streams while other calls run: every call has its own scratch memory."""
+    c, dev, table = _filled(amd, gpu, [9000], 2, 64, 128, seed=26)
+    table, lens = table.to(gpu), torch.tensor([9000], dtype=torch.int32, device=gpu)
+    qs = [torch.randn(1, 16, 128, generator=_gen(60 + i)).half().to(gpu) for i in range(8)]
+    x = torch.randn(700, 12, 128, generator=_gen(61)).half().to(gpu)
+    want = [amd.ops.attention_paged(q, dev, table, lens) for q in qs]
+    prompt = amd.ops.attention_prompt(x[:, :8], x[:, 8:10], x[:, 10:])
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(3)], [[], [], []]
+    for i in range(8):
+        for n, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[n].append(amd.ops.attention_prompt(x[:, :8], x[:, 8:10], x[:, 10:]) if n == 2 else amd.ops.attention_paged(qs[i], dev, table, lens))
+    torch.cuda.synchronize()
+    for i in range(8):
+        assert torch.equal(got[0][i], want[i]) and torch.equal(got[1][i], want[i]) and torch.equal(got[2][i], prompt)
 
 
 def test_results_do_not_depend_on_the_run(amd, gpu):
