@@ -160,6 +160,7 @@ __global__ __launch_bounds__(256, NQ == 4 ? 1 : 2) void attention_paged_kernel(c
     const int runs = (n_tiles + a.tiles_per_split - 1) / a.tiles_per_split;
     if (split > 0 && split >= runs) return;
     const int per_run = runs > 1 && runs <= a.n_splits ? ((n_tiles + runs - 1) / runs + 3) & ~3 : a.tiles_per_split;
+    const bool parts = runs > 1 && a.n_splits > 1;   // else this workgroup has the whole row
     const int t_lo = split * per_run;
     const int t_hi = n_tiles < t_lo + per_run ? n_tiles : t_lo + per_run;
 
@@ -462,7 +463,7 @@ __global__ __launch_bounds__(256, NQ == 4 ? 1 : 2) void attention_paged_kernel(c
         for (int ch = 4 * (threadIdx.x & 15); ch < d; ch += 64) {
             f32x4 x = {0.f, 0.f, 0.f, 0.f};
             for (int w = 0; w < 4; ++w) x += *o_at(w, row, ch);
-            if (a.n_splits > 1) {
+            if (parts) {
                 *reinterpret_cast<f32x4 *>(a.part_o + ((qrow * a.n_heads + head) * a.n_splits + split) * d + ch) = x;
             } else {
                 // a row without a key is 0
@@ -473,7 +474,7 @@ __global__ __launch_bounds__(256, NQ == 4 ? 1 : 2) void attention_paged_kernel(c
                 *reinterpret_cast<u32x2 *>((T *)a.out + qrow * a.o_tok + (int64_t)head * a.o_head + ch) = raw;
             }
         }
-        if (a.n_splits > 1 && (threadIdx.x & 15) == 0) {
+        if (parts && (threadIdx.x & 15) == 0) {
             float *ml = a.part_ml + ((qrow * a.n_heads + head) * a.n_splits + split) * 2;
             ml[0] = ma;
             ml[1] = sum;
@@ -504,7 +505,8 @@ __global__ __launch_bounds__(256) void attention_paged_join_kernel(const PagedAr
     }
     const int len = a.lens[b] < 0 ? 0 : (a.lens[b] > PA_MAX_LEN ? PA_MAX_LEN : a.lens[b]);
     const int wanted = ((len + 63) / 64 + a.tiles_per_split - 1) / a.tiles_per_split;
-    const int used = wanted < 1 ? 1 : (wanted > a.n_splits ? a.n_splits : wanted);
+    if (wanted <= 1) return;   // one run: the first kernel wrote the row
+    const int used = wanted > a.n_splits ? a.n_splits : wanted;
     if (tid < 64) {   // PA_MAX_SPLITS runs at most: one wave weighs them
         const float *ml = a.part_ml + (idx * a.n_splits + tid) * 2;
         const float mx = tid < used ? ml[0] : -INFINITY, l = tid < used ? ml[1] : 0.f;
