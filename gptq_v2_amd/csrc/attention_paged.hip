@@ -162,7 +162,10 @@ __global__ __launch_bounds__(256, NQ == 4 ? 1 : 2) void attention_paged_kernel(c
     const int per_run = runs > 1 && runs <= a.n_splits ? ((n_tiles + runs - 1) / runs + 3) & ~3 : a.tiles_per_split;
     const bool parts = runs > 1 && a.n_splits > 1;   // else this workgroup has the whole row
     const int t_lo = split * per_run;
-    const int t_hi = n_tiles < t_lo + per_run ? n_tiles : t_lo + per_run;
+    // (as far as the last of the workgroup's rows sees; a run may be empty for it)
+    const int last_tok = (it.tile * MR + MR - 1) / a.group, hidden = last_tok < it.n ? it.n - 1 - last_tok : 0;
+    const int vis = len > hidden ? len - hidden : 0, vis_tiles = (vis + 63) >> 6;
+    const int t_hi = vis_tiles < t_lo + per_run ? vis_tiles : t_lo + per_run;
 
     // the query rows go to LDS (registers are what the loads in flight need), 0 where there is no row or channel
     for (int i = threadIdx.x; i < MR * DP / 8; i += 256) {
@@ -182,7 +185,7 @@ __global__ __launch_bounds__(256, NQ == 4 ? 1 : 2) void attention_paged_kernel(c
     __syncthreads();
 
     // The pages of a tile, in scalar registers; the entries of the table are fetched a tile before they are used.
-    bool bad = runs > a.n_splits;   // a token that should be there lies on no page (the table ends within the runs)
+    bool bad = vis > a.table_width << a.page_log2;   // a token that should be there lies on no page
     const int32_t *table = a.table + (int64_t)it.b * a.table_width;
     struct Pages {
         int id[NP];
@@ -192,7 +195,7 @@ __global__ __launch_bounds__(256, NQ == 4 ? 1 : 2) void attention_paged_kernel(c
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
             const int tok = t * 64 + 16 * SUB * i, e = tok >> a.page_log2;
-            p.id[i] = tok < len && e < a.table_width ? pa_scalar_load(table, e) : -1;
+            p.id[i] = tok < vis && e < a.table_width ? pa_scalar_load(table, e) : -1;
         }
         return p;
     };
@@ -201,7 +204,7 @@ __global__ __launch_bounds__(256, NQ == 4 ? 1 : 2) void attention_paged_kernel(c
 #pragma unroll
         for (int i = 0; i < NP; ++i)
             if (p.id[i] < 0 || p.id[i] >= a.n_pages) {
-                bad |= t * 64 + 16 * SUB * i < len;
+                bad |= t * 64 + 16 * SUB * i < vis;
                 p.id[i] = 0;
             }
         return p;
@@ -260,8 +263,8 @@ __global__ __launch_bounds__(256, NQ == 4 ? 1 : 2) void attention_paged_kernel(c
 #pragma unroll
         for (int t2 = 0; t2 < DT; ++t2) o[nt][t2] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    // tokens from here on are hidden from some row: behind the sequence, or after a query token of it
-    const int partly = len - it.n + 1;
+    // tokens from here on are hidden from some row: behind the sequence, or after a query token of the workgroup's
+    const int partly = len - it.n + it.tile * MR / a.group + 1;
 
     int t = t_lo + wave;
     Pages next;
