@@ -115,13 +115,17 @@ __device__ __forceinline__ Item find_item(const PagedArgs &a, int item, int mr)
         const int b = item / tiles;
         return {b, item - b * tiles, b, 1};
     }
+    // the starts rise: the item's sequence is the last of those that start at or before it; 64 are looked at at a time
     const auto start = [&](int s) { return (int64_t)a.cu[s] * a.group / mr + s; };
-    int lo = 0, hi = a.batch - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (start(mid) <= item) lo = mid;
-        else hi = mid - 1;
+    const int lane = threadIdx.x & 63;
+    int lo = -1;
+    for (int b0 = 0; b0 < a.batch; b0 += 64) {
+        const int c = __popcll(__ballot(b0 + lane < a.batch && start(b0 + lane) <= item));
+        lo += c;
+        if (c < 64) break;
     }
+    if (lo < 0) return {0, 0, 0, 0};
+    lo = __builtin_amdgcn_readfirstlane(lo);
     const int64_t row0 = a.cu[lo], n = (int64_t)a.cu[lo + 1] - row0, tile = item - start(lo);
     if (row0 < 0 || n <= 0 || row0 + n > a.n_tokens || tile < 0 || tile * mr >= n * a.group) return {lo, 0, 0, 0};
     return {lo, (int)tile, row0, (int)n};
@@ -135,7 +139,7 @@ __device__ __forceinline__ int pa_value_swizzle(int R) { return (R >> 1) & 3; }
 
 // SUB: 16-token groups of a tile on one page (pages of 16, 32 and 64 or more: 1, 2, 4)
 template <typename T, int NC, int NQ, int SUB>
-__global__ __launch_bounds__(256, NQ == 4 ? 1 : 2) void attention_paged_kernel(const PagedArgs a)
+__global__ __launch_bounds__(256, 2) void attention_paged_kernel(const PagedArgs a)
 {
     typedef Mfma<T> MM;
     typedef typename MM::vec vec;
@@ -497,12 +501,13 @@ __global__ __launch_bounds__(256) void attention_paged_join_kernel(const PagedAr
     int b = (int)tok;
     if (a.cu) {
         if (tok < a.cu[0] || tok >= a.cu[a.batch]) return;   // behind the last sequence: left as it is
-        int lo = 0, hi = a.batch - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (a.cu[mid] <= tok) lo = mid;
-            else hi = mid - 1;
+        int lo = -1;
+        for (int b0 = 0; b0 < a.batch; b0 += 64) {
+            const int c = __popcll(__ballot(b0 + (tid & 63) < a.batch && a.cu[b0 + (tid & 63)] <= tok));
+            lo += c;
+            if (c < 64) break;
         }
+        lo = __builtin_amdgcn_readfirstlane(lo < 0 ? 0 : lo);
         b = lo;
         if (a.cu[b + 1] <= tok || a.cu[b] < 0 || a.cu[b + 1] > a.n_tokens) return;   // not rising: the first kernel left it out
     }
@@ -553,15 +558,16 @@ struct Plan {
     int64_t n_items;
 };
 
-// Query rows per workgroup: as many 16-row tiles as a sequence has rows on average, up to 4.  Runs: workgroups for two
-// rounds (512 run at once), of at least 256 tokens (one tile per wave), at most 64 of them; sequences of 4096, 2048 and 8192
-// tokens with twice as many: 112 against 108, 116 against 98, 111 against 107 us.
+// Query rows per workgroup: one or two 16-row tiles (four do not fit the registers of two waves a SIMD: 64 rows each of 8
+// sequences of 2048 took 64 us against 33, 512 tokens behind 7680 303 against 222).  Runs: workgroups for two rounds (512
+// run at once), of at least 256 tokens (one tile per wave), at most 64 of them; sequences of 4096, 2048 and 8192 tokens with
+// twice as many: 112 against 108, 116 against 98, 111 against 107 us.
 Plan paged_plan(int64_t n_tokens, int64_t batch, bool ragged, int64_t n_heads, int64_t n_kv_heads, int64_t page, int64_t table_width)
 {
     Plan p;
     const int64_t group = n_heads / n_kv_heads;
     const int64_t rows = ragged ? gq_cdiv(n_tokens * group, batch) : group;
-    p.nq = rows <= 16 ? 1 : (rows <= 32 ? 2 : 4);
+    p.nq = rows <= 16 ? 1 : 2;
     const int mr = 16 * p.nq;
     p.n_items = ragged ? n_tokens * group / mr + batch : batch * gq_cdiv(group, mr);
     const int64_t tiles = gq_cdiv(table_width * page, 64), wgs = p.n_items * n_kv_heads;
@@ -592,12 +598,10 @@ int launch_paged(const PagedArgs &a, const Plan &p, hipStream_t s)
     } while (0)
     if (a.head_dim <= 64) {
         if (p.nq == 1) GQ_PA(1, 1);
-        else if (p.nq == 2) GQ_PA(1, 2);
-        else GQ_PA(1, 4);
+        else GQ_PA(1, 2);
     } else {
         if (p.nq == 1) GQ_PA(2, 1);
-        else if (p.nq == 2) GQ_PA(2, 2);
-        else GQ_PA(2, 4);
+        else GQ_PA(2, 2);
     }
 #undef GQ_PA
     GQ_LAUNCH_CHECK();
