@@ -106,6 +106,7 @@ struct Item {
     int b, tile;
     int64_t row0;   // first query token's row in q
     int n;          // query tokens of the sequence; 0: nothing to do
+    int len;        // its cached tokens
 };
 
 __device__ __forceinline__ Item find_item(const PagedArgs &a, int item, int mr)
@@ -113,22 +114,28 @@ __device__ __forceinline__ Item find_item(const PagedArgs &a, int item, int mr)
     if (!a.cu) {
         const int tiles = (a.group + mr - 1) / mr;
         const int b = item / tiles;
-        return {b, item - b * tiles, b, 1};
+        return {b, item - b * tiles, b, 1, a.lens[b]};
     }
-    // the starts rise: the item's sequence is the last of those that start at or before it; 64 are looked at at a time
-    const auto start = [&](int s) { return (int64_t)a.cu[s] * a.group / mr + s; };
+    // The starts rise: the item's sequence is the last of those that start at or before it; 64 are looked at at a time, and
+    // what is wanted of it is nearly always in the lanes.
     const int lane = threadIdx.x & 63;
-    int lo = -1;
+    int lo = -1, c = 0, mine = 0, len = 0;
     for (int b0 = 0; b0 < a.batch; b0 += 64) {
-        const int c = __popcll(__ballot(b0 + lane < a.batch && start(b0 + lane) <= item));
+        const int at = b0 + lane < a.batch ? b0 + lane : a.batch;
+        mine = a.cu[at];
+        len = a.lens[at < a.batch ? at : a.batch - 1];
+        c = __popcll(__ballot(b0 + lane < a.batch && (int64_t)mine * a.group / mr + at <= item));
         lo += c;
         if (c < 64) break;
     }
-    if (lo < 0) return {0, 0, 0, 0};
+    if (lo < 0) return {0, 0, 0, 0, 0};
     lo = __builtin_amdgcn_readfirstlane(lo);
-    const int64_t row0 = a.cu[lo], n = (int64_t)a.cu[lo + 1] - row0, tile = item - start(lo);
-    if (row0 < 0 || n <= 0 || row0 + n > a.n_tokens || tile < 0 || tile * mr >= n * a.group) return {lo, 0, 0, 0};
-    return {lo, (int)tile, row0, (int)n};
+    c = __builtin_amdgcn_readfirstlane(c);
+    const bool here = c > 0 && c < 64;
+    const int64_t row0 = here ? __builtin_amdgcn_readlane(mine, c - 1) : a.cu[lo];
+    const int64_t n = (here ? __builtin_amdgcn_readlane(mine, c) : a.cu[lo + 1]) - row0, tile = item - (row0 * a.group / mr + lo);
+    if (row0 < 0 || n <= 0 || row0 + n > a.n_tokens || tile < 0 || tile * mr >= n * a.group) return {lo, 0, 0, 0, 0};
+    return {lo, (int)tile, row0, (int)n, here ? (int)__builtin_amdgcn_readlane(len, c - 1) : a.lens[lo]};
 }
 
 // Piece p (of 16 bytes) of the 128 bytes R of a buffer lies in place p ^ swizzle(R).  16 lanes read 16 pieces at a time
@@ -157,7 +164,7 @@ __global__ __launch_bounds__(256, 2) void attention_paged_kernel(const PagedArgs
     const Item it = find_item(a, blockIdx.x / a.n_kv_heads, MR);
     if (it.n == 0) return;
     const int d = a.head_dim, page = 1 << a.page_log2;
-    int len = a.lens[it.b];
+    int len = it.len;
     len = len < 0 ? 0 : (len > PA_MAX_LEN ? PA_MAX_LEN : len);   // (positions and the tile behind them stay below 2^31)
     const int n_tiles = (len + 63) >> 6;
     // runs of equal length, as many as runs of tiles_per_split take (so none is longer or empty)
@@ -221,27 +228,27 @@ __global__ __launch_bounds__(256, 2) void attention_paged_kernel(const PagedArgs
     };
     uint8_t *buf_k = sm_k[wave], *buf_v = sm_v[wave];
     // Copy j brings the pieces 64 j .. 64 j + 63 of the buffer, lane l piece l: of its 128 bytes R the piece that belongs
-    // there.  Channels behind head_dim are out of the descriptor's range and arrive as 0.
-    const auto copy_k = [&](int t, const Pages &p) {
+    // there.  Channels behind head_dim are out of the descriptor's range, wherever in a page the tile begins, and arrive as 0.
+    constexpr int ROWS = 1024 / DP;    // tokens of a copy of keys, all on one page
+    constexpr int PER = COPIES / NP;   // copies of a page's part of the tile's values: DP rows of SUB pieces
+    unsigned k_off[COPIES], v_off[COPIES];   // in the page, from the tile's first token in it
 #pragma unroll
-        for (int j = 0; j < COPIES; ++j) {
-            constexpr int ROWS = 1024 / DP;   // tokens of a copy, all on one page
-            const int piece = (lane & 7) ^ pa_key_swizzle<DP>(8 * j + (lane >> 3));
-            const int row = DP == 128 ? lane >> 3 : 2 * (lane >> 3) + (piece >> 2), ch = 16 * (DP == 128 ? piece : piece & 3);
-            const int tok = (t * 64 + ROWS * j) & (page - 1);
-            const int off = ch < d ? (tok + row) * d + ch : (int)0x80000000;
-            copy(a.k_codes, p.id[ROWS * j / (16 * SUB)], off, buf_k + 1024 * j);
-        }
+    for (int j = 0; j < COPIES; ++j) {
+        const int piece = (lane & 7) ^ pa_key_swizzle<DP>(8 * j + (lane >> 3));
+        const int row = DP == 128 ? lane >> 3 : 2 * (lane >> 3) + (piece >> 2), ch = 16 * (DP == 128 ? piece : piece & 3);
+        k_off[j] = ch < d ? ((ROWS * j) % (16 * SUB) + row) * d + ch : 0x80000000u;
+        const int q = 64 * (j % PER) + (lane & ~7) + ((lane & 7) ^ pa_value_swizzle(lane >> 3)), c = q / SUB;
+        v_off[j] = c < d ? c * page + 16 * (q % SUB) : 0x80000000u;
+    }
+    const auto copy_k = [&](int t, const Pages &p) {
+        const unsigned at = SUB == 4 ? ((t * 64) & (page - 1)) * d : 0;
+#pragma unroll
+        for (int j = 0; j < COPIES; ++j) copy(a.k_codes, p.id[ROWS * j / (16 * SUB)], (int)(k_off[j] + at), buf_k + 1024 * j);
     };
     const auto copy_v = [&](int t, const Pages &p) {
+        const unsigned at = SUB == 4 ? (t * 64) & (page - 1) : 0;
 #pragma unroll
-        for (int j = 0; j < COPIES; ++j) {
-            constexpr int PER = COPIES / NP;   // copies of a page's part of the tile: DP rows of SUB pieces
-            const int q = 64 * (j % PER) + (lane & ~7) + ((lane & 7) ^ pa_value_swizzle(lane >> 3));
-            const int row = q / SUB, tok = ((t * 64 + 16 * SUB * (j / PER)) & (page - 1)) + 16 * (q % SUB);
-            const int off = row < d ? row * page + tok : (int)0x80000000;
-            copy(a.v_codes, p.id[j / PER], off, buf_v + 1024 * j);
-        }
+        for (int j = 0; j < COPIES; ++j) copy(a.v_codes, p.id[j / PER], (int)(v_off[j] + at), buf_v + 1024 * j);
     };
     float ks, vs, ks_next, vs_next;
     const auto load_scales = [&](const Pages &p) {
