@@ -21,10 +21,10 @@
 //
 // Bound by HBM: 2 head_dim bytes per cached token and kv head.  A long sequence is cut into runs of tokens for several
 // workgroups, whose (O, M, l) a second kernel joins.
-// Measured at 64 heads on 8, 128 channels, pages of 64: one token each of 64 sequences of 391 to 8192 134 us (4.8 TB/s),
-// of 128 sequences of 2048 98 us (5.5 TB/s); four tokens of one sequence of 131071 74 us (3.6 TB/s, the join 5.5 us of it: the
+// Measured at 64 heads on 8, 128 channels, pages of 64: one token each of 64 sequences of 391 to 8192 131 us (5.0 TB/s),
+// of 128 sequences of 2048 98 us (5.5 TB/s); four tokens of one sequence of 131071 72 us (3.7 TB/s, the join 5.5 us of it: the
 // copies alone take 43 us, and the decoding, products and exponentials of 32 query rows hide behind them only in part);
-// 100 tokens 6.2 us (a launch).
+// 512 tokens behind 7680 199 us (669 TFLOP/s); 100 tokens of 32 heads 5.8 us (a launch).
 #include <type_traits>
 
 #include "gq_common.h"
