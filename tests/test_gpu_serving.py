@@ -445,6 +445,30 @@ def test_paged_attention_of_many_ragged_sequences(amd, gpu):
     _check_paged(got, q, c, table, lens, new, torch.float16)
 
 
+@pytest.mark.parametrize("lens,new,hq,hkv,page", [([1500], [1490], 4, 1, 64), ([40, 900, 20], [33, 700, 20], 8, 4, 16), ([1300, 64], [1300, 1], 2, 1, 128)])
+def test_paged_attention_of_chunks_in_runs(amd, gpu, lens, new, hq, hkv, page):
+    """Chunks whose first rows see none of the later runs of their sequence, and workgroups that end inside a token's heads."""
+    c, dev, table = _filled(amd, gpu, lens, hkv, page, 64, seed=27, spread=2.0)
+    q = torch.randn(sum(new), hq, 64, generator=_gen(54)).to(torch.bfloat16)
+    got = amd.ops.attention_paged(q.to(gpu), dev, table.to(gpu), torch.tensor(lens, dtype=torch.int32, device=gpu), _cu(new, gpu))
+    _check_paged(got, q, c, table, lens, new, torch.bfloat16)
+
+
+def test_paged_attention_of_a_chunk_with_a_missing_page(amd, gpu):
+    """Rows that see the missing page, or a token behind the table, are NaN; another sequence is as ever."""
+    lens, new = [300, 100], [200, 3]
+    c, dev, table = _filled(amd, gpu, lens, 1, 16, 64, seed=28)
+    q = torch.randn(203, 4, 64, generator=_gen(55)).half()
+    bad = table.clone()
+    bad[0, 17] = -1   # tokens 272..287: rows from 172 on
+    got = amd.ops.attention_paged(q.to(gpu), dev, bad.to(gpu), torch.tensor(lens, dtype=torch.int32, device=gpu), _cu(new, gpu)).cpu()
+    assert torch.isnan(got[172:200]).all()
+    _check_paged(got[200:], q[200:], c, table[1:], lens[1:], new[1:], torch.float16)
+    got = amd.ops.attention_paged(q.to(gpu), dev, table[:, :18].contiguous().to(gpu), torch.tensor(lens, dtype=torch.int32, device=gpu), _cu(new, gpu)).cpu()
+    assert torch.isnan(got[188:200]).all()
+    _check_paged(got[200:], q[200:], c, table[1:], lens[1:], new[1:], torch.float16)
+
+
 def test_paged_attention_of_shared_pages(amd, gpu):
     """Sequences that begin with the same pages, and one that names a page twice."""
     c, dev, table = _filled(amd, gpu, [128, 128, 128], 2, 64, 64, seed=25)
