@@ -627,7 +627,8 @@ def attention_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     """Attention over whole prompts: q (tokens, heads, head_dim), k / v (tokens, kv heads, head_dim) in fp16 or bf16, head_dim
     a multiple of 8 up to 128; strided views (slices of a merged q/k/v product) are taken as they are.  ``cu_seqlens``
     (sequences + 1) int32 says where the packed sequences begin and end (None: one sequence); rows behind the last are left
-    as they are.  Causal: token i of a sequence sees tokens 0..i.  ``scale`` defaults to head_dim ** -0.5."""
+    as they are.  Causal: token i of a sequence sees tokens 0..i.  ``scale`` defaults to head_dim ** -0.5.
+    ``out`` must not overlap q, k or v."""
     return _serving.attention_prompt(q, k, v, cu_seqlens, causal, scale, out)
 
 
@@ -649,7 +650,8 @@ def attention_paged(q: torch.Tensor, cache: PagedCache, block_table: torch.Tenso
     (sequences) int32 of them with the query tokens included: its n query tokens are its last n, each sees the keys up to its
     own position.  ``cu_seqlens`` None: one query token for each sequence (a decoder's step); several are a checked
     draft or a chunk of a prompt behind its cached beginning.  A row that sees nothing is 0; one that sees a token on no page
-    is NaN (its sequence's others may be).  The scratch memory of long sequences comes from torch's allocator, a tensor per call."""
+    is NaN (its sequence's others may be).  The scratch memory of long sequences comes from torch's allocator, a tensor per call.
+    ``out`` must not overlap q."""
     return _serving.attention_paged(q, *cache, block_table, seq_lens, cu_seqlens, scale, out)
 
 
