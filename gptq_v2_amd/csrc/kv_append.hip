@@ -15,10 +15,12 @@
 // store, and nobody else may touch the page while codes are re-expressed.  The input stays in registers between the two.
 // A thread takes 16 channels of each of two tokens of keys -- the two halves of 8 rotated pairs, one angle for both -- or 4
 // tokens x 8 channels of values, whose codes go through LDS so that both the loads (by token) and the stores (by channel)
-// are whole lines.
+// are whole lines.  Rotary widths that are no multiple of 16 share a head out by the same 16 channels an item, see any_pairs.
 // Bound by HBM for prompts (16-bit input in, one byte out), next to the vector instructions of rotation and rounding (74 %
 // busy): 4.2 TB/s, 111 us for 8 ragged prompts of 11314 tokens in all, 32 query heads on 32 of 128 channels; by a launch and
 // dependent loads for single tokens (64 sequences: 6.8 us).
+#include <type_traits>
+
 #include "gq_common.h"
 
 namespace {
@@ -101,6 +103,106 @@ __device__ __forceinline__ void load_pair(const T *head, int p, const float *cos
     }
 }
 
+// Any other even rotary width (a kernel of its own: the pairs' second sides are at no aligned place then).  Item p of a head
+// takes r = half - 8 p (0 to 8) of the pairs (8 p + i, 8 p + i + half); where pairs end inside its 16 channels the places
+// left take channels that are not rotated, so that the items share the head out among them:
+//   a_i: channel 8 p + i where i < r, else 16 p + 8 + i;   b_i: channel (r > 0 ? 8 p + half : 16 p) + i
+// (half = 8 P + r for the item P where pairs end: its b goes on into the channels from 2 half = 16 P + 2 r on, its a takes
+// the last 8 - r before 16 P + 16).  Of interleaved pairs a and b are the item's two runs of 8.  The second sides are loaded
+// and stored at the alignment of an element, which the memory unit takes.  Single tokens take the launch's time as ever; 8
+// ragged prompts of 11314 tokens of 32/32 heads of 80: 119 us at a width of 40, 92 at 32 and at 48 (interleaved 106), of 128
+// channels 164 at 72, 111 at 64.
+__device__ __forceinline__ int any_pairs(int p, int half)
+{
+    const int r = half - 8 * p;
+    return r < 0 ? 0 : (r > 8 ? 8 : r);
+}
+
+struct AnyPlaces {
+    int r, split, a, b;   // pairs; elements of a that lie at 8 p, where the rest of it and b lie
+};
+
+__device__ __forceinline__ AnyPlaces any_places(int p, int half, int interleaved)
+{
+    const int r = any_pairs(p, half);
+    if (interleaved) return {r, 0, 16 * p, 16 * p + 8};
+    return {r, r, 16 * p + 8, r > 0 ? 8 * p + half : 16 * p};
+}
+
+template <typename T>
+__device__ __forceinline__ void load8f_any(const T *p, float (&f)[8])
+{
+    T v[8];
+    __builtin_memcpy(v, p, sizeof(v));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = static_cast<float>(v[i]);
+}
+
+template <typename T>
+__device__ __forceinline__ void load_pair_any(const T *head, int p, const float *cos_r, const float *sin_r, int half, int interleaved, bool last_row,
+                                              float (&a)[8], float (&b)[8])
+{
+    const AnyPlaces at = any_places(p, half, interleaved);
+    if (at.split < 8) load8f(head + at.a, a);
+    if (at.split > 0) {
+        float x[8];
+        load8f(head + 8 * p, x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) a[i] = i < at.split ? x[i] : a[i];
+    }
+    load8f_any(head + at.b, b);
+    if (at.r == 0) return;
+    float c[8], s[8];
+    if (at.r == 8 || !last_row) {   // (8 angles also where fewer are left: the next row's follow, but not behind the table's last)
+        __builtin_memcpy(c, cos_r + 8 * p, sizeof(c));
+        __builtin_memcpy(s, sin_r + 8 * p, sizeof(s));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            c[i] = i < at.r ? cos_r[8 * p + i] : 0.f;
+            s[i] = i < at.r ? sin_r[8 * p + i] : 0.f;
+        }
+    }
+    const auto turn = [&](int i, float &x, float &y) {
+        if (i >= at.r) return;
+        const float u = x, v = y;
+        x = __fsub_rn(__fmul_rn(u, c[i]), __fmul_rn(v, s[i]));
+        y = __fadd_rn(__fmul_rn(v, c[i]), __fmul_rn(u, s[i]));
+    };
+    if (interleaved) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            turn(i, a[2 * i], a[2 * i + 1]);
+            turn(4 + i, b[2 * i], b[2 * i + 1]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) turn(i, a[i], b[i]);
+    }
+}
+
+// 8 elements each for the places of a and b in a head's row
+template <typename E>
+__device__ __forceinline__ void store_pair_any(E *row, int p, int half, int interleaved, const E (&a)[8], const E (&b)[8])
+{
+    const AnyPlaces at = any_places(p, half, interleaved);
+    if (at.split == 0) {
+        __builtin_memcpy(row + at.a, a, sizeof(a));
+    } else if (at.split == 8) {
+        __builtin_memcpy(row + 8 * p, a, sizeof(a));
+    } else {
+        const auto pieces = [&](auto width) {
+            constexpr int W = decltype(width)::value;
+#pragma unroll
+            for (int i = 0; i < 8; i += W) __builtin_memcpy(row + (i < at.split ? 8 * p : at.a) + i, a + i, W * sizeof(E));
+        };
+        if (at.split % 4 == 0) pieces(std::integral_constant<int, 4>());
+        else if (at.split % 2 == 0) pieces(std::integral_constant<int, 2>());
+        else pieces(std::integral_constant<int, 1>());
+    }
+    __builtin_memcpy(row + at.b, b, sizeof(b));
+}
+
 __device__ __forceinline__ unsigned to_codes4(float a, float b, float c, float d)
 {
     // infinities saturate (the conversion would make them NaN); NaN stays NaN
@@ -139,7 +241,8 @@ __device__ __forceinline__ int find_sequence(int batch, int64_t pos, F f)
     return __builtin_amdgcn_readfirstlane(n) - 1;
 }
 
-template <typename T>
+// ANY: the rotary width is no multiple of 16
+template <typename T, bool ANY>
 __device__ __forceinline__ void append_page(const AppendArgs &a, int item, int head, bool is_v, unsigned *sm_max, unsigned *sm_tile)
 {
     const int tid = threadIdx.x, nt = blockDim.x;
@@ -210,8 +313,10 @@ __device__ __forceinline__ void append_page(const AppendArgs &a, int item, int h
             if (it < n_keys) {
                 const int s = s0 + it / n_pairs;
                 const int64_t at = (first + s) * (a.rot >> 1);
-                load_pair(x + (row_of_0 + s) * tok_stride, it % n_pairs, a.cos_t + at, a.sin_t + at, a.rot, a.interleaved,
-                          *reinterpret_cast<float (*)[8]>(&f[k][0]), *reinterpret_cast<float (*)[8]>(&f[k][8]));
+                float (&lo)[8] = *reinterpret_cast<float (*)[8]>(&f[k][0]), (&hi)[8] = *reinterpret_cast<float (*)[8]>(&f[k][8]);
+                const T *row = x + (row_of_0 + s) * tok_stride;
+                if constexpr (ANY) load_pair_any(row, it % n_pairs, a.cos_t + at, a.sin_t + at, a.rot >> 1, a.interleaved, first + s >= a.max_pos - 1, lo, hi);
+                else load_pair(row, it % n_pairs, a.cos_t + at, a.sin_t + at, a.rot, a.interleaved, lo, hi);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) measure(f[k][i]);
             }
@@ -262,17 +367,21 @@ __device__ __forceinline__ void append_page(const AppendArgs &a, int item, int h
         for (int k = 0; k < 2; ++k) {
             const int it = tid + k * nt;
             if (it < n_keys) {
-                int lo, hi;
-                pair_channels(it % n_pairs, a.rot, a.interleaved, lo, hi);
                 uint8_t *row = codes + (s0 + it / n_pairs) * d;
                 const float (&g)[16] = f[k];
-                u32x2 w;
-                w[0] = to_codes4(g[0] * inv, g[1] * inv, g[2] * inv, g[3] * inv);
-                w[1] = to_codes4(g[4] * inv, g[5] * inv, g[6] * inv, g[7] * inv);
-                *reinterpret_cast<u32x2 *>(row + lo) = w;
-                w[0] = to_codes4(g[8] * inv, g[9] * inv, g[10] * inv, g[11] * inv);
-                w[1] = to_codes4(g[12] * inv, g[13] * inv, g[14] * inv, g[15] * inv);
-                *reinterpret_cast<u32x2 *>(row + hi) = w;
+                const u32x2 wa = {to_codes4(g[0] * inv, g[1] * inv, g[2] * inv, g[3] * inv), to_codes4(g[4] * inv, g[5] * inv, g[6] * inv, g[7] * inv)};
+                const u32x2 wb = {to_codes4(g[8] * inv, g[9] * inv, g[10] * inv, g[11] * inv), to_codes4(g[12] * inv, g[13] * inv, g[14] * inv, g[15] * inv)};
+                if constexpr (ANY) {
+                    uint8_t ca[8], cb[8];
+                    __builtin_memcpy(ca, &wa, 8);
+                    __builtin_memcpy(cb, &wb, 8);
+                    store_pair_any(row, it % n_pairs, a.rot >> 1, a.interleaved, ca, cb);
+                } else {
+                    int lo, hi;
+                    pair_channels(it % n_pairs, a.rot, a.interleaved, lo, hi);
+                    *reinterpret_cast<u32x2 *>(row + lo) = wa;
+                    *reinterpret_cast<u32x2 *>(row + hi) = wb;
+                }
             }
         }
         return;
@@ -317,7 +426,7 @@ __device__ __forceinline__ void append_page(const AppendArgs &a, int item, int h
 }
 
 // The query rows of a token, or part of its heads: a thread takes 16 channels, both sides of a rotated pair, so that q_out may be q.
-template <typename T>
+template <typename T, bool ANY>
 __device__ __forceinline__ void rotate_query(const AppendArgs &a, int64_t token, int part)
 {
     int64_t pos;
@@ -330,25 +439,37 @@ __device__ __forceinline__ void rotate_query(const AppendArgs &a, int64_t token,
         pos = a.past[token];
     }
     const bool known = pos >= 0 && pos < a.max_pos;
-    const int64_t at = (known ? pos : 0) * (a.rot >> 1);
+    const int64_t angle = known ? pos : 0, at = angle * (a.rot >> 1);
     const int n_pairs = a.head_dim >> 4, n = a.n_heads * n_pairs;
     for (int i = part * blockDim.x + threadIdx.x; i < n; i += a.q_parts * blockDim.x) {
         const int head = i / n_pairs, p = i - head * n_pairs;
         float lo[8], hi[8];
-        load_pair((const T *)a.q + token * a.q_tok + head * a.q_head, p, a.cos_t + at, a.sin_t + at, a.rot, a.interleaved, lo, hi);
+        const T *x = (const T *)a.q + token * a.q_tok + head * a.q_head;
+        if constexpr (ANY) load_pair_any(x, p, a.cos_t + at, a.sin_t + at, a.rot >> 1, a.interleaved, angle >= a.max_pos - 1, lo, hi);
+        else load_pair(x, p, a.cos_t + at, a.sin_t + at, a.rot, a.interleaved, lo, hi);
         if (!known) {
 #pragma unroll
             for (int k = 0; k < 8; ++k) lo[k] = hi[k] = NAN;
         }
-        int cl, chh;
-        pair_channels(p, a.rot, a.interleaved, cl, chh);
         T *y = (T *)a.q_out + token * a.qo_tok + head * a.qo_head;
-        store8f(y + cl, lo);
-        store8f(y + chh, hi);
+        if constexpr (ANY) {
+            T ya[8], yb[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                ya[k] = static_cast<T>(lo[k]);
+                yb[k] = static_cast<T>(hi[k]);
+            }
+            store_pair_any(y, p, a.rot >> 1, a.interleaved, ya, yb);
+        } else {
+            int cl, chh;
+            pair_channels(p, a.rot, a.interleaved, cl, chh);
+            store8f(y + cl, lo);
+            store8f(y + chh, hi);
+        }
     }
 }
 
-template <typename T>
+template <typename T, bool ANY>
 __global__ __launch_bounds__(512) void kv_append_kernel(const AppendArgs a)
 {
     __shared__ unsigned sm_max[8];
@@ -356,10 +477,10 @@ __global__ __launch_bounds__(512) void kv_append_kernel(const AppendArgs a)
     const unsigned n_kv = (unsigned)a.n_items * a.n_kv_heads * 2;
     if (blockIdx.x < n_kv) {
         const unsigned ih = blockIdx.x >> 1, item = ih / a.n_kv_heads;
-        append_page<T>(a, (int)item, (int)(ih - item * a.n_kv_heads), blockIdx.x & 1, sm_max, sm_tile);
+        append_page<T, ANY>(a, (int)item, (int)(ih - item * a.n_kv_heads), blockIdx.x & 1, sm_max, sm_tile);
     } else {
         const unsigned i = blockIdx.x - n_kv, token = i / a.q_parts;
-        rotate_query<T>(a, token, (int)(i - token * a.q_parts));
+        rotate_query<T, ANY>(a, token, (int)(i - token * a.q_parts));
     }
 }
 
@@ -383,8 +504,9 @@ extern "C" int gq_kv_append(const gq_kv_append_args *args, gq_stream_t stream)
     GQ_REQUIRE(n_kv_heads > 0 && n_pages >= 0 && n_tokens >= 0 && batch >= 0 && table_width >= 0, "gq_kv_append: negative size");
     GQ_REQUIRE(batch < (1 << 24) && n_tokens < ((int64_t)1 << 31) && n_kv_heads <= 65536 && n_heads <= 65536, "gq_kv_append: too many tokens, sequences or heads");
     GQ_REQUIRE(cu_seqlens || n_tokens == batch, "gq_kv_append: %lld tokens for %lld sequences need cu_seqlens", (long long)n_tokens, (long long)batch);
-    GQ_REQUIRE(rotary_dim >= 0 && rotary_dim <= head_dim && rotary_dim % 16 == 0, "gq_kv_append: rotary_dim %lld is not a multiple of 16 up to head_dim",
-               (long long)rotary_dim);
+    GQ_REQUIRE(rotary_dim == 0 || (rotary_dim >= 16 && rotary_dim <= head_dim && rotary_dim % 2 == 0),
+               "gq_kv_append: rotary_dim %lld is neither 0 nor an even number from 16 to head_dim", (long long)rotary_dim);
+    const bool any = rotary_dim % 16 != 0;
     if (n_tokens == 0 || batch == 0) return GQ_OK;
     GQ_REQUIRE(cache.k_codes && cache.v_codes && cache.k_scale && cache.v_scale && k.data && v.data && block_table && past_lens, "gq_kv_append: NULL pointer");
     GQ_REQUIRE(!rotary_dim || (cos_t && sin_t && max_pos > 0), "gq_kv_append: a rotation needs the tables of cosines and sines");
@@ -393,8 +515,9 @@ extern "C" int gq_kv_append(const gq_kv_append_args *args, gq_stream_t stream)
                    (!q.data || (q.token_stride % 8 == 0 && q.head_stride % 8 == 0 && q_out.token_stride % 8 == 0 && q_out.head_stride % 8 == 0)),
                "gq_kv_append: strides must be multiples of 8 elements");
     GQ_REQUIRE(!q.data || gq_rows_apart(q_out, n_tokens, n_heads, head_dim), "gq_kv_append: rows of q_out overlap");
-    GQ_REQUIRE((((uintptr_t)cache.k_codes | (uintptr_t)cache.v_codes | (uintptr_t)k.data | (uintptr_t)v.data | (uintptr_t)q.data | (uintptr_t)q_out.data | (uintptr_t)cos_t |
-                 (uintptr_t)sin_t) & 15) == 0, "gq_kv_append: pointers must be 16-byte aligned");
+    GQ_REQUIRE((((uintptr_t)cache.k_codes | (uintptr_t)cache.v_codes | (uintptr_t)k.data | (uintptr_t)v.data | (uintptr_t)q.data | (uintptr_t)q_out.data) & 15) == 0 &&
+                   (((uintptr_t)cos_t | (uintptr_t)sin_t) & (any ? 3 : 15)) == 0,
+               "gq_kv_append: pointers must be 16-byte aligned (the tables' 4 where rotary_dim is no multiple of 16)");
     AppendArgs a;
     a.q = q.data, a.k = k.data, a.v = v.data, a.q_out = q_out.data;
     a.q_tok = q.token_stride, a.q_head = q.head_stride, a.qo_tok = q_out.token_stride, a.qo_head = q_out.head_stride;
@@ -415,8 +538,15 @@ extern "C" int gq_kv_append(const gq_kv_append_args *args, gq_stream_t stream)
     const int64_t grid = n_items * n_kv_heads * 2 + q_blocks;
     GQ_REQUIRE(grid < GQ_MAX_THREADS / threads, "gq_kv_append: too many tokens for one call");
     a.n_items = (int)n_items;
-    if (dtype == GQ_F16) hipLaunchKernelGGL(kv_append_kernel<_Float16>, dim3((unsigned)grid), dim3(threads), lds, (hipStream_t)stream, a);
-    else hipLaunchKernelGGL(kv_append_kernel<__bf16>, dim3((unsigned)grid), dim3(threads), lds, (hipStream_t)stream, a);
+#define GQ_KA(T, ANY) hipLaunchKernelGGL((kv_append_kernel<T, ANY>), dim3((unsigned)grid), dim3(threads), lds, (hipStream_t)stream, a)
+    if (dtype == GQ_F16) {
+        if (any) GQ_KA(_Float16, true);
+        else GQ_KA(_Float16, false);
+    } else {
+        if (any) GQ_KA(__bf16, true);
+        else GQ_KA(__bf16, false);
+    }
+#undef GQ_KA
     GQ_LAUNCH_CHECK();
     return GQ_OK;
 }

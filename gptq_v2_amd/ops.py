@@ -638,9 +638,9 @@ def kv_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, block_table: 
     """Appends the new tokens' keys and values, k / v (tokens, kv heads, head_dim) in fp16 or bf16, to the cache, behind the
     ``past_lens`` (sequences) int32 tokens that each sequence has; ``block_table`` (sequences, width) int32 names its pages.
     ``cu_seqlens`` None: one new token for each sequence.  With ``cos`` / ``sin`` (positions, rotary_dim / 2) fp32 the keys are
-    rotated on the way, and q (tokens, heads, head_dim), if given, into ``q_out`` (which may be q), which is returned; pairs of
-    channels are (j, j + rotary_dim / 2), or (2j, 2j + 1) if ``interleaved``.  See gq_kv_append in gptq_amd.h for the scales
-    and for tokens without a page or an angle."""
+    rotated on the way (rotary_dim even, 16 to head_dim), and q (tokens, heads, head_dim), if given, into ``q_out`` (which may
+    be q), which is returned; pairs of channels are (j, j + rotary_dim / 2), or (2j, 2j + 1) if ``interleaved``.  See
+    gq_kv_append in gptq_amd.h for the scales and for tokens without a page or an angle."""
     return _serving.kv_append(*cache, k, v, block_table, past_lens, cu_seqlens, q, cos, sin, interleaved, q_out)
 
 

@@ -446,7 +446,7 @@ int gq_attention_prompt(const gq_attention_prompt_args *args, gq_stream_t stream
  * page already holds tokens of the sequence its scale does not fall, and they are re-expressed when it grows.  Infinities
  * saturate, NaN stays NaN.  Slots behind the new tokens stay as they are.  No page may be appended to by two sequences of a call.
  * cu_seqlens NULL: one new token per sequence (n_tokens == batch).
- * Rotation of the first rotary_dim channels (a multiple of 16; 0: none) by position p = past_lens[b] + i with
+ * Rotation of the first rotary_dim channels (an even number from 16 on; 0: none) by position p = past_lens[b] + i with
  * cos / sin [max_pos][rotary_dim / 2] fp32: channel pairs (j, j + rotary_dim / 2), or (2j, 2j + 1) if interleaved,
  *   a' = a cos - b sin,  b' = b cos + a sin,  each operation rounded to fp32.
  * q (may be NULL) is rotated the same way into q_out (may be q), rounded once to `dtype`.
