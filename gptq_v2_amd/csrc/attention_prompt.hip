@@ -321,9 +321,11 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void attention_prompt_kernel
     l += __shfl_xor(l, 32, 64);
     const float inv = 1.f / l;
     // A lane holds 4 adjacent channels here and there of its row: through LDS (the wave's 32 rows, places as in the tiles),
-    // so that rows are written in whole lines.
+    // so that rows are written in whole lines.  Two waves' rows fill a buffer of keys.
+    constexpr int OUT = 32 * DP;
+    static_assert(2 * OUT <= AP_K * DP && AP_Q == 4 * 32, "the rows of four waves fit the two buffers of keys");
     __syncthreads();
-    T *so = sm_k0 + wave * 32 * DP;
+    T *so = (wave < 2 ? sm_k0 : sm_k1) + (wave & 1) * OUT;
 #pragma unroll
     for (int t = 0; t < DT; ++t)
 #pragma unroll
