@@ -43,11 +43,13 @@ template <typename T> struct Mma;
 template <> struct Mma<_Float16> {
     typedef f16x8 vec;
     static constexpr unsigned EXPONENT_ONE = 0x04000400u;
+    static constexpr float LIFT = 7.f;
     static __device__ __forceinline__ f32x16 run(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 };
 template <> struct Mma<__bf16> {
     typedef bf16x8 vec;
     static constexpr unsigned EXPONENT_ONE = 0x00800080u;
+    static constexpr float LIFT = 0.f;
     static __device__ __forceinline__ f32x16 run(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 };
 
@@ -203,9 +205,12 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void attention_prompt_kernel
 #pragma unroll
             for (int r = 0; r < 16; ++r) top = fmaxf(top, s[tb][r]);
         top = gq_max_xor32(top) * a.scale;
-        // The weights are 2^(s - mx) for an mx that follows the row's maximum only when that is more than 8 above it: up to
-        // 256 instead of 1, which costs them no precision, and O is rescaled once or twice a row instead of in most tiles
-        // (one of the wave's 32 rows finds a new maximum in nearly every tile; 4 x 2048 tokens 189 -> 180 us).
+        // The weights are 2^(s - mx + LIFT) for an mx that follows the row's maximum only when that is more than 8 above it:
+        // O is rescaled once or twice a row instead of in most tiles (one of the wave's 32 rows finds a new maximum in nearly
+        // every tile; 4 x 2048 tokens 189 -> 180 us).  They meet the values in the values' type, the matrix instruction's one
+        // type for both, rounded once (11 bits in fp16, 8 in bf16); l sums them unrounded.  fp16 has 11 bits down to 2^-14 and
+        // steps of 2^-24 below: LIFT = 7 uses the range up to 2^15 (of 65504), so that a weight 2^-21 of the row's largest
+        // keeps its bits and what falls below half a step is 2^-32 of it, nothing even a million times over.
         if (__any(top > mx + 8.f)) {
             const float to = fmaxf(top, mx);
             const float f = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - to);
@@ -216,7 +221,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void attention_prompt_kernel
 #pragma unroll
                 for (int r = 0; r < 16; ++r) o[t][r] *= f;
         }
-        const float ref = mx == -INFINITY ? 0.f : mx;
+        const float ref = mx == -INFINITY ? 0.f : mx - Mma<T>::LIFT;
         vec p[4];
 #pragma unroll
         for (int tb = 0; tb < 2; ++tb)
