@@ -1,10 +1,16 @@
 // Attention of a few query tokens per sequence over a paged cache of 8-bit keys and values (the layout and the scales
 // that kv_append.hip writes): a decoder's step for one new token, or for the several of a checked draft or a chunk.
 //
-// With K = ks[page] k8 and V = vs[page] v8, in powers of two (c = softmax scale * log2 e):
-//   y_t = c ks (q . k8_t) + log2 vs,  M = max y,  w_t = 2^(y_t - M),  O = sum_t w_t v8_t / sum_t w_t / vs
-// The value's scale sits in the exponent, so the weights that meet the codes on the matrix core are at most 1 whatever
-// the scales are, and the denominator takes it out again in 32 bits.
+// With K = ks[page] k8 and V = vs[page] v8, in powers of two (c = softmax scale * log2 e), and any whole number e per page:
+//   y_t = c ks (q . k8_t) + log2 vs - e,  w_t = 2^(y_t - M + 7),  O = sum_t w_t (2^e v8_t) / sum_t w_t 2^e / vs
+// for a reference M near max y.  2^e v8 is exact in fp16 for e from -15 (the smallest code is 2^-9) to 7 (the largest 448),
+// and costs nothing: the conversion of codes takes a factor.  So e is the scale's own exponent less that of the first page the
+// wave sees, as far as that range goes: within it w_t is the softmax weight alone and small scales cost it nothing; what lies
+// outside stays in the exponent y, and the denominator takes it out again in 32 bits.
+// The weights meet the codes on the matrix core in fp16, rounded once (11 bits, against 8 in bf16); the denominator sums them
+// unrounded.  fp16 has 11 bits down to 2^-14 and steps of 2^-24 below.  M lags up to 8 behind the maximum (see there), so the
+// largest weight of a row is 2^7 to 2^15 (of 65504): a weight keeps its bits down to 2^-21 of it, and what is lost below is
+// 2^-32 of it.
 //
 // A wave takes 64 tokens at a time: S^T = K Q^T (16 x 16 x 32 tiles: tokens by query rows) and O^T = V^T P^T.  Row
 // 4 g + i of the S^T tile a stands for token 16 g + 4 a + i; lane group g then holds, as the tiles' results, the weights of
@@ -16,13 +22,12 @@
 // nobody: the next tile's keys are under way as soon as this one's have met the queries, its values after this one's
 // have met the weights.
 // The rows are the query heads that share a kv head (times the tokens of the sequence); the cache is read once for
-// every 16 NQ of them.  e4m3 codes are exact in either 16-bit type: Q K^T runs in q's type, P V in fp16 (w <= 1 keeps
-// 11 bits there, against 8 in bf16).
+// every 16 NQ of them.  e4m3 codes are exact in either 16-bit type: Q K^T runs in q's type.
 //
 // Bound by HBM: 2 head_dim bytes per cached token and kv head.  A long sequence is cut into runs of tokens for several
 // workgroups, whose (O, M, l) a second kernel joins.
 // Measured at 64 heads on 8, 128 channels, pages of 64: one token each of 64 sequences of 391 to 8192 131 us (5.0 TB/s),
-// of 128 sequences of 2048 98 us (5.5 TB/s); four tokens of one sequence of 131071 72 us (3.7 TB/s, the join 5.5 us of it: the
+// of 128 sequences of 2048 98 us (5.5 TB/s); four tokens of one sequence of 131071 73.5 us (3.65 TB/s, the join 5.5 us of it: the
 // copies alone take 43 us, and the decoding, products and exponentials of 32 query rows hide behind them only in part);
 // 512 tokens behind 7680 199 us (669 TFLOP/s); 100 tokens of 32 heads 5.8 us (a launch).
 #include <type_traits>
@@ -33,6 +38,7 @@ namespace {
 
 constexpr int PA_MAX_SPLITS = 64;   // one wave weighs them
 constexpr int PA_MAX_LEN = 1 << 30;     // longest sequence; tables are narrower (a longer one is NaN)
+constexpr int PA_NO_EXPONENT = 1000;
 constexpr float PA_LOG2E = 1.44269504088896340736f;
 
 struct PagedArgs {
@@ -57,6 +63,8 @@ __device__ __forceinline__ V pa_scalar_load(const V *p, int64_t i)
     return *(const V __attribute__((address_space(4))) *)(uintptr_t)(p + i);
 }
 
+__device__ __forceinline__ int pa_exponent(float x) { return (int)(__float_as_uint(x) >> 23 & 0xff) - 127; }
+
 // At most N of the wave's copies are left under way; the oldest end first.
 template <int N>
 __device__ __forceinline__ void pa_wait()
@@ -80,11 +88,11 @@ template <typename T> struct Mfma;
 template <> struct Mfma<_Float16> {
     typedef f16x8 vec;
     static __device__ __forceinline__ f32x4 run(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
-    // 8 codes (two words) to the operand's type, exactly
-    static __device__ __forceinline__ f16x8 decode(unsigned lo, unsigned hi)
+    // 8 codes (two words) times a power of two from 2^-15 to 2^7 to the operand's type, exactly
+    static __device__ __forceinline__ f16x8 decode(unsigned lo, unsigned hi, float f = 1.f)
     {
-        const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, false), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, true);
-        const f16x2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, false), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, true);
+        const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, f, false), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, f, true);
+        const f16x2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, f, false), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, f, true);
         return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
     }
 };
@@ -278,6 +286,7 @@ __global__ __launch_bounds__(256, 2) void attention_paged_kernel(const PagedArgs
     const int partly = len - it.n + it.tile * MR / a.group + 1;
 
     int t = t_lo + wave;
+    int e0 = PA_NO_EXPONENT;   // of the first page's value scale, to which the others' are set in relation (any number is right)
     Pages next;
 #pragma unroll
     for (int i = 0; i < NP; ++i) next.id[i] = 0;
@@ -331,7 +340,15 @@ __global__ __launch_bounds__(256, 2) void attention_paged_kernel(const PagedArgs
             load_scales(now);
         }
         vs = fmaxf(vs, 0x1p-100f);   // a scale of 0 must not become an infinite weight
-        const float mul = a.scale * ks, add = __builtin_amdgcn_logf(vs), inv = 1.f / vs;
+        int e = pa_exponent(vs);
+        if (e0 == PA_NO_EXPONENT) {   // (here, where the scale has long arrived: before the loop it cost single tokens 0.3 us)
+            e0 = __builtin_amdgcn_readfirstlane(e);
+            e0 = e0 < -80 ? -80 : (e0 > 100 ? 100 : e0);   // the scale of a page of zeros is 2^-100: 2^e / vs stays far from 2^128
+        }
+        e -= e0;
+        e = e < -15 ? -15 : (e > 7 ? 7 : e);
+        const float unit = __uint_as_float((unsigned)(e + 127) << 23);
+        const float mul = a.scale * ks, add = __builtin_amdgcn_logf(vs) - (float)e, inv = unit / vs;
         f16x8 p[NQ][2];
 #pragma unroll
         for (int nt = 0; nt < NQ; ++nt) {
@@ -348,8 +365,8 @@ __global__ __launch_bounds__(256, 2) void attention_paged_kernel(const PagedArgs
                 }
             if constexpr (!masked) top = fmaf(top, mul, add);   // (a lane's tokens have one scale, and it is positive)
             top = gq_max_xor32(gq_max_xor16(top));
-            // M follows the maximum only when that is more than 2^8 above it: weights up to 256 instead of 1, and O is
-            // rescaled in a wave's first tile instead of in most (some row of 16 finds a new maximum in nearly every one)
+            // M follows the maximum only when that is more than 8 above it: O is rescaled in a wave's first tile instead of in
+            // most (some row of 16 finds a new maximum in nearly every one)
             if (__any(top > mx[nt] + 8.f)) {
                 const float to = fmaxf(top, mx[nt]);
                 const float f = mx[nt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx[nt] - to);
@@ -360,7 +377,7 @@ __global__ __launch_bounds__(256, 2) void attention_paged_kernel(const PagedArgs
 #pragma unroll
                     for (int j = 0; j < 4; ++j) o[nt][t2][j] *= f;
             }
-            const float ref = mx[nt] == -INFINITY ? 0.f : mx[nt];
+            const float ref = mx[nt] == -INFINITY ? 0.f : mx[nt] - 7.f;
             float sum = 0.f;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
@@ -403,7 +420,7 @@ __global__ __launch_bounds__(256, 2) void attention_paged_kernel(const PagedArgs
             for (int t2 = 0; t2 < DT; ++t2) {
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    const f16x8 vf = Mfma<_Float16>::decode(vr[t2][2 * u], vr[t2][2 * u + 1]);
+                    const f16x8 vf = Mfma<_Float16>::decode(vr[t2][2 * u], vr[t2][2 * u + 1], unit);
 #pragma unroll
                     for (int nt = 0; nt < NQ; ++nt) o[nt][t2] = Mfma<_Float16>::run(vf, p[nt][u], o[nt][t2]);
                 }
@@ -420,8 +437,8 @@ __global__ __launch_bounds__(256, 2) void attention_paged_kernel(const PagedArgs
                         w[i] = (tok >> 4) == g && ((tok >> 2) & 3) == i ? vr[t2][i] & (0xffu << (8 * (tok & 3))) : 0u;
 #pragma unroll
                     for (int nt = 0; nt < NQ; ++nt) {
-                        f32x4 x = Mfma<_Float16>::run(Mfma<_Float16>::decode(w[0], w[1]), p[nt][0], f32x4{0.f, 0.f, 0.f, 0.f});
-                        x = Mfma<_Float16>::run(Mfma<_Float16>::decode(w[2], w[3]), p[nt][1], x);
+                        f32x4 x = Mfma<_Float16>::run(Mfma<_Float16>::decode(w[0], w[1], unit), p[nt][0], f32x4{0.f, 0.f, 0.f, 0.f});
+                        x = Mfma<_Float16>::run(Mfma<_Float16>::decode(w[2], w[3], unit), p[nt][1], x);
                         if (t * 64 + tok <= last[nt]) o[nt][t2] += x;
                     }
                 }
