@@ -339,7 +339,7 @@ __global__ __launch_bounds__(256, 2) void attention_paged_kernel(const PagedArgs
             copy_k(t + 4, now);
             load_scales(now);
         }
-        vs = fmaxf(vs, 0x1p-100f);   // a scale of 0 must not become an infinite weight
+        vs = vs < 0x1p-100f ? 0x1p-100f : vs;   // a scale of 0 must not become an infinite weight, one that is NaN stays it
         int e = pa_exponent(vs);
         if (e0 == PA_NO_EXPONENT) {   // (here, where the scale has long arrived: before the loop it cost single tokens 0.3 us)
             e0 = __builtin_amdgcn_readfirstlane(e);
@@ -387,7 +387,8 @@ __global__ __launch_bounds__(256, 2) void attention_paged_kernel(const PagedArgs
                     sum += w;
                     p[nt][i >> 1][4 * (i & 1) + j] = (_Float16)w;
                 }
-            l[nt] = fmaf(sum, inv, l[nt]);
+            // (where a lane sees none of its tokens, their page's scale may be anything, NaN too)
+            l[nt] = masked && sum == 0.f ? l[nt] : fmaf(sum, inv, l[nt]);
         }
         if (more) pa_wait<COPIES>();   // the values are there: the next keys may be under way
         else pa_wait<0>();

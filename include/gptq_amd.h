@@ -467,7 +467,9 @@ int gq_kv_append(const gq_kv_append_args *args, gq_stream_t stream);
 
 /* Attention of each sequence's query tokens over its cached keys and values: the n query tokens of sequence b are the last
  * n of its seq_lens[b], and each sees the keys up to its own position (a row that sees none is 0).  cu_seqlens NULL: one
- * query token per sequence.  Any positive scales are taken; products in fp32, the weights rounded to fp16 for the second.
+ * query token per sequence.  Any positive scales are taken (value scales below 2^-100 count as 2^-100, the smallest that
+ * gq_kv_append gives); products in fp32, the weights rounded to fp16 for the second.  A row that sees a token of a page whose
+ * scale is NaN is NaN.
  * A row that sees a token on no page, or behind its sequence's table, is NaN; the sequence's other rows may be.
  * gq_attention_paged_workspace: bytes of scratch memory a call of these sizes needs (0: none); ragged = cu_seqlens given. */
 size_t gq_attention_paged_workspace(int64_t n_tokens, int64_t batch, int ragged, int n_heads, int n_kv_heads, int head_dim, int page,
