@@ -334,12 +334,13 @@ __device__ __forceinline__ void append_page(const AppendArgs &a, int item, int h
     }
     int e = exponent_for(most);
     if (s0 > 0) {
-        // the tokens already there keep the scale from falling; a scale that is no power of two is rounded up to one
+        // the tokens already there keep the scale from falling; a scale that is no power of two is rounded up to one, and one
+        // that is no number leaves them NaN
         const unsigned ob = __float_as_uint(old);
         int eo = old > 0.f && old < INFINITY ? (int)(ob >> 23) - 127 + ((ob & 0x7fffff) != 0) : MIN_EXP;
         eo = eo < MIN_EXP ? MIN_EXP : (eo > MAX_EXP ? MAX_EXP : eo);
         e = eo > e ? eo : e;
-        const float ratio = old > 0.f && old < INFINITY ? old * pow2f(-e) : 0.f;
+        const float ratio = old > 0.f && old < INFINITY ? old * pow2f(-e) : (old <= 0.f ? 0.f : NAN);
         if (ratio != 1.f) {
             if (is_v) {
                 const int words = (s0 + 3) >> 2;

@@ -650,8 +650,8 @@ def attention_paged(q: torch.Tensor, cache: PagedCache, block_table: torch.Tenso
     (sequences) int32 of them with the query tokens included: its n query tokens are its last n, each sees the keys up to its
     own position.  ``cu_seqlens`` None: one query token for each sequence (a decoder's step); several are a checked
     draft or a chunk of a prompt behind its cached beginning.  A row that sees nothing is 0; one that sees a token on no page
-    is NaN (its sequence's others may be), and so is one that sees a token of a page whose scale is NaN.  The scratch memory of long sequences comes from torch's allocator, a tensor per call.
-    ``out`` must not overlap q."""
+    is NaN (its sequence's others may be), and so is one that sees a token of a page whose scale is NaN.  The scratch memory
+    of long sequences comes from torch's allocator, a tensor per call.  ``out`` must not overlap q."""
     return _serving.attention_paged(q, *cache, block_table, seq_lens, cu_seqlens, scale, out)
 
 

@@ -443,8 +443,8 @@ int gq_attention_prompt(const gq_attention_prompt_args *args, gq_stream_t stream
 /*
  * gq_kv_append writes the new tokens of each sequence behind the past_lens[b] it has: the keys rotated, both in e4m3
  * at the page's scale, 2^e with the smallest e (at least -100) for which the page's finite magnitudes fit 448 2^e.  When a
- * page already holds tokens of the sequence its scale does not fall, and they are re-expressed when it grows.  Infinities
- * saturate, NaN stays NaN.  Slots behind the new tokens stay as they are.  No page may be appended to by two sequences of a call.
+ * page already holds tokens of the sequence its scale does not fall, and they are re-expressed when it grows (to NaN where
+ * that scale is not finite).  Infinities saturate, NaN stays NaN.  Slots behind the new tokens stay as they are.  No page may be appended to by two sequences of a call.
  * cu_seqlens NULL: one new token per sequence (n_tokens == batch).
  * Rotation of the first rotary_dim channels (an even number from 16 on; 0: none) by position p = past_lens[b] + i with
  * cos / sin [max_pos][rotary_dim / 2] fp32: channel pairs (j, j + rotary_dim / 2), or (2j, 2j + 1) if interleaved,

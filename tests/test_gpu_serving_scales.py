@@ -56,3 +56,27 @@ def test_paged_scales_from_the_smallest_on(amd, gpu):
     lens = torch.tensor([90], dtype=torch.int32, device=gpu)
     outs = [amd.ops.attention_paged(q, dev._replace(v_scale=torch.full_like(dev.v_scale, s)), table.to(gpu), lens) for s in (2.0 ** -100, 0.0, 1e-40, 2.0 ** -120)]
     assert all(torch.equal(outs[0], x) for x in outs[1:]) and (outs[0] != 0).any()
+
+
+@pytest.mark.parametrize("bad", [math.nan, -math.nan, math.inf])
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_append_to_a_page_of_a_damaged_scale(amd, gpu, bad, which):
+    """The tokens that the page holds become NaN, the new one and the other head's are what they would be anyway."""
+    gen = _gen(37)
+    pools = [amd.ops.PagedCache.empty(1, 2, 16, 32, gpu) for _ in range(2)]
+    k, v = torch.randn(6, 2, 32, generator=gen).half().to(gpu), torch.randn(6, 2, 32, generator=gen).half().to(gpu)
+    table = torch.zeros(1, 1, dtype=torch.int32, device=gpu)
+    past = lambda n: torch.tensor([n], dtype=torch.int32, device=gpu)   # noqa: E731
+    for i, dev in enumerate(pools):
+        amd.ops.kv_append(dev, k[:5], v[:5], table, past(0), _cu([5], gpu))
+        if i:
+            getattr(dev, which + "_scale")[0, 1] = bad
+        amd.ops.kv_append(dev, k[5:] * 64, v[5:] * 64, table, past(5))   # (a larger scale than before, so that both ways end at one)
+    tokens = [tuple(x.float().cpu() for x in (dev.k, dev.v.transpose(2, 3))) for dev in pools]
+    for name, a, b in zip("kv", *tokens):
+        if name == which:
+            assert torch.isnan(b[0, 1, :5]).all()
+            b[0, 1, :5] = a[0, 1, :5]
+        assert torch.equal(a, b)
+    for a, b in zip(pools[0][2:], pools[1][2:]):
+        assert torch.equal(a, b)
