@@ -1,5 +1,6 @@
-"""Builds gptq_v2_amd/lib/libgptq_amd.so (hipcc, gfx950 only).  Run as a script,
-`python gptq_v2_amd/build.py`: importing the package needs the library this produces."""
+"""Builds gptq_v2_amd/lib/libgptq_amd.so (hipcc, gfx950 only) and the torch binding of the serving operators (g++).  Run as a
+script, `python gptq_v2_amd/build.py`: importing the package needs the library this produces; the binding is needed by the
+serving operators alone, and a failure to build it is raised when the library is there."""
 import os
 import shutil
 import subprocess
@@ -20,6 +21,7 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=o
 
 
 BINDING = os.path.join(HERE, "_serving_binding.so")
+STAMP = os.path.join(OBJ, "serving_binding.stamp")   # what BINDING was built with
 
 
 def _binding_cmd() -> list:
@@ -49,6 +51,28 @@ def _stale(out: str, deps) -> bool:
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def _binding_stamp(cmd) -> str:
+    """The binding is compiled against torch's C++ headers and Python's: another of either wants another binding."""
+    import sysconfig
+    import torch
+    return "\n".join([torch.__version__, str(sysconfig.get_config_var("SOABI")), *cmd])
+
+
+def _binding_stale(stamp: str) -> bool:
+    if not os.path.exists(STAMP) or open(STAMP).read() != stamp:
+        return True
+    return _stale(BINDING, [os.path.join(CSRC, "serving_binding.cpp"), os.path.join(ROOT, "include", "gptq_amd.h")])
+
+
+def _build_binding(force: bool, run) -> None:
+    cmd = _binding_cmd()
+    stamp = _binding_stamp(cmd)
+    if force or _binding_stale(stamp):
+        run(cmd)
+        with open(STAMP, "w") as f:
+            f.write(stamp)
+
+
 def build(force: bool = False, verbose: bool = True) -> str:
     os.makedirs(OBJ, exist_ok=True)
     os.makedirs(os.path.dirname(LIB), exist_ok=True)
@@ -70,13 +94,12 @@ def build(force: bool = False, verbose: bool = True) -> str:
             print(" ".join(cmd), flush=True)
         subprocess.check_call(cmd)
 
-    binding = []
-    if force or _stale(BINDING, [os.path.join(CSRC, "serving_binding.cpp"), os.path.join(ROOT, "include", "gptq_amd.h")]):
-        binding = [_binding_cmd()]
-    with ThreadPoolExecutor(max_workers=min(8, max(1, len(jobs) + len(binding)))) as ex:
-        list(ex.map(run, binding + jobs))
-    if jobs or force or _stale(LIB, objs):
-        run([hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB, *objs])
+    with ThreadPoolExecutor(max_workers=min(8, len(jobs) + 1)) as ex:
+        binding = ex.submit(_build_binding, force, run)
+        list(ex.map(run, jobs))
+        if jobs or force or _stale(LIB, objs):
+            run([hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB, *objs])
+        binding.result()
     return LIB
 
 

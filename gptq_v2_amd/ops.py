@@ -611,7 +611,11 @@ class TokenLogprobs(NamedTuple):
 def _load_binding():
     """The C++ binding of these operators (csrc/serving_binding.cpp: checks, outputs and the call, where checks in Python
     would take longer than the kernels), on the entries of the library that ``_lib`` has loaded."""
-    from . import _serving_binding as b
+    try:
+        from . import _serving_binding as b
+    except ImportError as e:
+        raise ImportError(f"the binding of the serving operators, gptq_v2_amd/_serving_binding.so, is missing or was built for another torch or Python: "
+                          f"build it with `python gptq_v2_amd/build.py` ({e})") from e
     lib = _lib.load()
     address = lambda name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value  # noqa: E731
     b.bind(address("gq_attention_prompt"), address("gq_kv_append"), address("gq_attention_paged_workspace"), address("gq_attention_paged"),
@@ -619,7 +623,19 @@ def _load_binding():
     return b
 
 
-_serving = _load_binding()
+class _Serving:
+    """The binding, loaded when the first of its operators is called: the others do without it."""
+
+    def __getattr__(self, name):
+        if name.startswith("__"):
+            raise AttributeError(name)
+        b = _load_binding()
+        for f in ("attention_prompt", "kv_append", "attention_paged", "token_logprobs"):
+            setattr(self, f, getattr(b, f))
+        return getattr(b, name)
+
+
+_serving = _Serving()
 
 
 def attention_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None, causal: bool = True,
