@@ -9,6 +9,7 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -57,12 +58,25 @@ const at::Tensor &tensor(PyObject *o, const char *name)
 // an undefined tensor for None
 at::Tensor optional_tensor(PyObject *o, const char *name) { return o == Py_None ? at::Tensor() : tensor(o, name); }
 
+// Neither kind of derivative passes through these operators: tensors that carry one are refused, not cut off silently.
 void no_grad(std::initializer_list<const at::Tensor *> ts)
 {
-    if (!at::GradMode::is_enabled()) return;
-    for (const at::Tensor *t : ts)
-        if (t->defined() && t->requires_grad())
+    const bool back = at::GradMode::is_enabled(), forth = c10::AutogradState::get_tls_state().get_fw_grad_mode();
+    if (!back && !forth) return;
+    for (const at::Tensor *t : ts) {
+        if (!t->defined()) continue;
+        if (back && t->requires_grad())
             raise(PyExc_RuntimeError, "this operator has no backward pass: call it under torch.no_grad() or on detached tensors");
+        if (forth && t->unsafeGetTensorImpl()->autograd_meta() && t->_fw_grad(0).defined())
+            raise(PyExc_RuntimeError, "this operator has no forward derivative: call it on tensors without a tangent");
+    }
+}
+
+// A caller's tensor that a kernel has written: its version rises, as by any in-place operation, so that what was saved or
+// kept of its old contents is known to be stale.
+void written(const at::Tensor &t)
+{
+    if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
 int64_t half_code(const at::Tensor &t)
@@ -137,6 +151,7 @@ gq_paged_cache cache_of(PyObject *const *o, const at::Tensor &like)
     dense(v, "cache.v", at::kFloat8_e4m3fn, 4, like);
     dense(ks, "cache.k_scale", at::kFloat, 2, like);
     dense(vs, "cache.v_scale", at::kFloat, 2, like);
+    no_grad({&k, &v, &ks, &vs});
     const int64_t n = k.size(0), h = k.size(1), page = k.size(2), d = k.size(3);
     if (v.size(0) != n || v.size(1) != h || v.size(2) != d || v.size(3) != page || ks.size(0) != n || ks.size(1) != h || vs.sizes() != ks.sizes())
         raise(PyExc_ValueError, "the cache's tensors do not belong together");
@@ -213,6 +228,7 @@ PyObject *attention_prompt(PyObject *, PyObject *const *o, Py_ssize_t n)
         no_grad({&out});
         a.out = rows_of(out), a.q = rows_of(q), a.k = rows_of(k), a.v = rows_of(v);
         call(c_prompt, a, "gq_attention_prompt", q);
+        written(out);
         return THPVariable_Wrap(out);
     });
 }
@@ -224,7 +240,7 @@ PyObject *kv_append(PyObject *, PyObject *const *o, Py_ssize_t n)
         expect(n, 14);
         const at::Tensor &k = tensor(o[4], "k"), &v = tensor(o[5], "v");
         const at::Tensor q = optional_tensor(o[9], "q"), cos = optional_tensor(o[10], "cos"), sin = optional_tensor(o[11], "sin");
-        no_grad({&k, &v, &q});
+        no_grad({&k, &v, &q, &cos, &sin});
         rows(k, "k");
         rows(v, "v", &k);
         gq_kv_append_args a = {};
@@ -262,6 +278,8 @@ PyObject *kv_append(PyObject *, PyObject *const *o, Py_ssize_t n)
         }
         a.k = rows_of(k), a.v = rows_of(v), a.q = rows_of(q), a.q_out = rows_of(q_out);
         call(c_append, a, "gq_kv_append", k);
+        for (int i = 0; i < 4; ++i) written(tensor(o[i], "cache"));
+        written(q_out);
         if (!q_out.defined()) Py_RETURN_NONE;
         return THPVariable_Wrap(q_out);
     });
@@ -303,6 +321,7 @@ PyObject *attention_paged(PyObject *, PyObject *const *o, Py_ssize_t n)
             a.workspace = scratch.data_ptr(), a.workspace_bytes = (int64_t)need;
         }
         call(c_paged, a, "gq_attention_paged", q);
+        written(out);
         return THPVariable_Wrap(out);
     });
 }

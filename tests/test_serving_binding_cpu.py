@@ -87,3 +87,39 @@ def test_a_failing_binding_leaves_the_library(tmp_path, monkeypatch):
     with pytest.raises(RuntimeError, match="no g"):
         b.build(force=True, verbose=False)
     assert ran[-1][-len(b.SOURCES) - 1] == b.LIB and len(ran) == len(b.SOURCES) + 1
+
+
+def _wrappers():
+    """Each operator as a function of its differentiable inputs (CPU tensors: the next check would refuse them)."""
+    import torch
+    from gptq_v2_amd import ops
+    table, lens = torch.zeros(4, 2, dtype=torch.int32), torch.ones(4, dtype=torch.int32)
+    cache = ops.PagedCache.empty(4, 2, 16, 64, "cpu")
+    q, k, cos = torch.zeros(4, 4, 64).half(), torch.zeros(4, 2, 64).half(), torch.zeros(9, 32)
+    return {
+        "prompt q": (q, lambda x: ops.attention_prompt(x, k, k)), "prompt k": (k, lambda x: ops.attention_prompt(q, x, k)),
+        "prompt v": (k, lambda x: ops.attention_prompt(q, k, x)), "append k": (k, lambda x: ops.kv_append(cache, x, k, table, lens)),
+        "append q": (q, lambda x: ops.kv_append(cache, k, k, table, lens, q=x, cos=cos, sin=cos)),
+        "append cos": (cos, lambda x: ops.kv_append(cache, k, k, table, lens, cos=x, sin=cos)),
+        "append sin": (cos, lambda x: ops.kv_append(cache, k, k, table, lens, cos=cos, sin=x)),
+        "paged q": (q, lambda x: ops.attention_paged(x, cache, table, lens)),
+        "logits": (torch.zeros(4, 9), lambda x: ops.token_logprobs(x, torch.zeros(4, dtype=torch.int64))),
+    }
+
+
+@pytest.mark.parametrize("name", ["prompt q", "prompt k", "prompt v", "append k", "append q", "append cos", "append sin", "paged q", "logits"])
+def test_tensors_that_carry_a_derivative_are_refused(name):
+    import torch
+    from torch.autograd import forward_ad
+    x, call = _wrappers()[name]
+    with pytest.raises(RuntimeError, match="no backward"):
+        call(x.clone().requires_grad_())
+    with torch.no_grad(), pytest.raises(ValueError, match="GPU"):
+        call(x.clone().requires_grad_())
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="no forward derivative"):
+                call(dual)
+        with pytest.raises(ValueError, match="GPU"):
+            call(forward_ad.unpack_dual(dual).primal)
