@@ -26,10 +26,10 @@
 //
 // Bound by HBM: 2 head_dim bytes per cached token and kv head.  A long sequence is cut into runs of tokens for several
 // workgroups, whose (O, M, l) a second kernel joins.
-// Measured at 64 heads on 8, 128 channels, pages of 64: one token each of 64 sequences of 391 to 8192 131 us (5.0 TB/s),
-// of 128 sequences of 2048 98 us (5.5 TB/s); four tokens of one sequence of 131071 73.5 us (3.65 TB/s, the join 5.5 us of it: the
-// copies alone take 43 us, and the decoding, products and exponentials of 32 query rows hide behind them only in part);
-// 512 tokens behind 7680 199 us (669 TFLOP/s); 100 tokens of 32 heads 5.8 us (a launch).
+// Measured at 64 heads on 8, 128 channels, pages of 64, on operands that no cache holds: one token each of 64 sequences of 391
+// to 8192 131 us (5.0 TB/s), of 128 sequences of 2048 98 us (5.5 TB/s); four tokens of one sequence of 131071 73.5 us (3.65
+// TB/s, the join 5.5 us of it: the copies alone take 43 us, and the decoding, products and exponentials of 32 query rows hide
+// behind them only in part); 100 tokens of 32 heads 5.9 us (a launch).  On cached operands 512 tokens behind 7680 200 us (667 TFLOP/s).
 #include <type_traits>
 
 #include "gq_common.h"
@@ -305,7 +305,7 @@ __global__ __launch_bounds__(256, 2) void attention_paged_kernel(const PagedArgs
         if (t + 8 < t_hi) next = fetch_pages(t + 8);
         // the keys are there: the values' copies may still be under way
         pa_wait<COPIES>();
-        __builtin_amdgcn_s_setprio(1);   // a wave at its products goes before one at its exponentials (1 x 131071: 67 -> 66 us)
+        __builtin_amdgcn_s_setprio(1);   // a wave at its products goes before one at its exponentials (1 x 131071: 74.2 -> 73.4 us)
         f32x4 s[NQ][4];
 #pragma unroll
         for (int nt = 0; nt < NQ; ++nt)
@@ -366,7 +366,7 @@ __global__ __launch_bounds__(256, 2) void attention_paged_kernel(const PagedArgs
             if constexpr (!masked) top = fmaf(top, mul, add);   // (a lane's tokens have one scale, and it is positive)
             top = gq_max_xor32(gq_max_xor16(top));
             // M follows the maximum only when that is more than 8 above it: O is rescaled in a wave's first tile instead of in
-            // most (some row of 16 finds a new maximum in nearly every one)
+            // most (some row of 16 finds a new maximum in nearly every one; 1 x 131071: 74.5 -> 74.1 us)
             if (__any(top > mx[nt] + 8.f)) {
                 const float to = fmaxf(top, mx[nt]);
                 const float f = mx[nt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx[nt] - to);
@@ -583,10 +583,14 @@ struct Plan {
     int64_t n_items;
 };
 
-// Query rows per workgroup: one or two 16-row tiles (four do not fit the registers of two waves a SIMD: 64 rows each of 8
-// sequences of 2048 took 64 us against 33, 512 tokens behind 7680 303 against 222).  Runs: workgroups for two rounds (512
-// run at once), of at least 256 tokens (one tile per wave), at most 64 of them; sequences of 4096, 2048 and 8192 tokens with
-// twice as many: 112 against 108, 116 against 98, 111 against 107 us.
+// Query rows per workgroup: one or two 16-row tiles (four do not fit the registers of two waves a SIMD).  Two where there are
+// more rows than one holds: 512 tokens behind 7680 with one and with two tiles 274 and 199 us, four tokens of one sequence of
+// 131071 75.2 and 73.7; on batches that one tile reads often enough two cost a little (8 sequences of 2048 with eight tokens
+// each 30.2 and 33).  One for 16 rows or fewer: 16 tokens of 8 sequences of 2048, 32 heads of their own, 35.4 and 42.3, single
+// tokens 131 and 145.
+// Runs: workgroups for two rounds (512 run at once), of at least 256 tokens (one tile per wave), at most 64 of them.  Sequences of
+// 4096, 2048 and 8192 tokens 108, 98 and 107 us; with twice as many 113, 115 and 110, with half as many 97, 98 and 105; 64 of
+// 391 to 8192 tokens 132, 132 and 129 (operands that no cache holds).
 Plan paged_plan(int64_t n_tokens, int64_t batch, bool ragged, int64_t n_heads, int64_t n_kv_heads, int64_t page, int64_t table_width)
 {
     Plan p;

@@ -15,8 +15,9 @@
 // Bound by the matrix core next to the softmax's vector instructions: 4 head_dim flops per visible (query, key) pair and
 // one exponential; for sequences of a few thousand tokens also by a workgroup's queries and outputs (64 KB at 128 channels,
 // which the other workgroup of a CU has to hide).  Measured with 128 channels, causal, on operands that no cache holds:
-// 16384 tokens of 32/8 heads 1950 us (1127 TFLOP/s, 0.9 of what a library product of 8192^3 reaches), 4 x 2048 tokens of
-// 32 heads 176 us (783 TFLOP/s, 1.5 TB/s), packed sequences of 1 to 3001 tokens 329 us (837 TFLOP/s), 77 tokens 6.5 us (a launch).
+// 16384 tokens of 32/8 heads 1940 us (1133 TFLOP/s, 0.9 of what a library product of 8192^3 reaches), 4 x 2048 tokens of
+// 32 heads 176 us (783 TFLOP/s, 1.5 TB/s: of the busy CUs' time the matrix pipe takes 47 %, the vector unit 52 %), packed
+// sequences of 1 to 3001 tokens 323 to 340 us (830 TFLOP/s), 77 tokens 6.5 us (a launch).
 #include <type_traits>
 
 #include "gq_common.h"
@@ -63,8 +64,8 @@ __device__ __forceinline__ int ap_swizzle(int row)
     return DP == 128 ? ((row & 3) << 2) | ((row >> 2) & 3) : (DP == 96 ? (row >> 2) & 3 : ((row & 2) << 1) | ((row >> 2) & 3));
 }
 
-// 3 workgroups to a CU where the registers allow it (up to 64 channels: 4 x 2048 tokens of 32/8 heads 111 -> 103 us, 8192
-// tokens not causal 603 -> 582), else 2.
+// 3 workgroups to a CU where the registers allow it (up to 64 channels: 4 x 2048 tokens of 32/8 heads 110 -> 102 us, 8192
+// tokens not causal 584 -> 567, on cached operands), else 2.
 template <typename T, int DP>
 __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void attention_prompt_kernel(const PromptArgs a)
 {
@@ -207,7 +208,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void attention_prompt_kernel
         top = gq_max_xor32(top) * a.scale;
         // The weights are 2^(s - mx + LIFT) for an mx that follows the row's maximum only when that is more than 8 above it:
         // O is rescaled once or twice a row instead of in most tiles (one of the wave's 32 rows finds a new maximum in nearly
-        // every tile; 4 x 2048 tokens 189 -> 180 us).  They meet the values in the values' type, the matrix instruction's one
+        // every tile; 4 x 2048 tokens 183.5 -> 175.5 us).  They meet the values in the values' type, the matrix instruction's one
         // type for both, rounded once (11 bits in fp16, 8 in bf16); l sums them unrounded.  fp16 has 11 bits down to 2^-14 and
         // steps of 2^-24 below: LIFT = 7 uses the range up to 2^15 (of 65504), so that a weight 2^-21 of the row's largest
         // keeps its bits and what falls below half a step is 2^-32 of it, nothing even a million times over.

@@ -17,8 +17,8 @@
 // tokens x 8 channels of values, whose codes go through LDS so that both the loads (by token) and the stores (by channel)
 // are whole lines.  Rotary widths that are no multiple of 16 share a head out by the same 16 channels an item, see any_pairs.
 // Bound by HBM for prompts (16-bit input in, one byte out), next to the vector instructions of rotation and rounding (74 %
-// busy): 4.2 TB/s, 111 us for 8 ragged prompts of 11314 tokens in all, 32 query heads on 32 of 128 channels; by a launch and
-// dependent loads for single tokens (64 sequences: 6.8 us).
+// of the busy CUs' time): 4.2 TB/s, 111 us for 8 ragged prompts of 11314 tokens in all, 32 query heads on 32 of 128 channels,
+// on operands that no cache holds; by a launch and dependent loads for single tokens (64 sequences: 6.7 us).
 #include <type_traits>
 
 #include "gq_common.h"
@@ -110,8 +110,8 @@ __device__ __forceinline__ void load_pair(const T *head, int p, const float *cos
 // (half = 8 P + r for the item P where pairs end: its b goes on into the channels from 2 half = 16 P + 2 r on, its a takes
 // the last 8 - r before 16 P + 16).  Of interleaved pairs a and b are the item's two runs of 8.  The second sides are loaded
 // and stored at the alignment of an element, which the memory unit takes.  Single tokens take the launch's time as ever; 8
-// ragged prompts of 11314 tokens of 32/32 heads of 80: 119 us at a width of 40, 92 at 32 and at 48 (interleaved 106), of 128
-// channels 164 at 72, 111 at 64.
+// ragged prompts of 11314 tokens of 32/32 heads of 80 (cached operands): 119 us at a width of 40, 92 at 32 and at 48
+// (interleaved 106), of 128 channels 164 at 72, 111 at 64.
 __device__ __forceinline__ int any_pairs(int p, int half)
 {
     const int r = half - 8 * p;

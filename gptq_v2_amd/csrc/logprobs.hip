@@ -16,8 +16,9 @@
 // in one 64-bit word, so ties go to the lowest index; a thread's largest counts with the last index of its chunk, which
 // can only lower the bound.
 //
-// Bound by HBM: rows * vocab elements in, a few words out.  4096 x 50272 bf16 with ten alternatives 89 us (4.6 TB/s; a read
-// alone reaches 6), one row of 32000 fp16 with five 7.6 us (a launch and four dependent steps).
+// Bound by HBM: rows * vocab elements in, a few words out; next to the vector instructions (86 % of the busy CUs' time).  4096 x
+// 50272 bf16 with ten alternatives 89 us (4.6 TB/s; a read alone reaches 6), one row of 32000 fp16 with five 7.6 us (a launch and
+// four dependent steps), on operands that no cache holds.
 #include <type_traits>
 
 #include "gq_common.h"
@@ -327,8 +328,11 @@ int launch_logprobs(const void *logits, int64_t n_rows, int64_t row_stride, int6
 #define GQ_LP(NT)                                                                                                                      \
     hipLaunchKernelGGL((token_logprobs_kernel<T, NT>), dim3((unsigned)n_rows), dim3(NT), 0, s, (const T *)logits, row_stride, (int)vocab, \
                        tokens, ignore_index, logprob, entropy, top, top_logprob, top_token)
-    // 16 waves a row where rows are few and have a chunk or two for each thread (1 x 32000 fp16: 7.8 us), 4 waves where the
-    // rows fill the chip by themselves (4096 x 50272 bf16: 87 us; 8 waves 89, 16 waves 157)
+    // 16 waves a row up to 512 rows that have a chunk or two for each thread (two such workgroups a CU at once), else 4.  16
+    // and 4 waves on operands that no cache holds, in us: 50272 words of bf16 with ten alternatives 10.9 and 16.6 for 64 rows,
+    // 12.1 and 17.8 for 256, 16.1 and 18.9 for 300, 18.0 and 20.8 for 512, 25.2 and 24.2 for 640, 32.2 and 30.9 for 1024; 17000
+    // words 12.2 and 11.7 for 512 rows, 21.6 and 14.7 for 1024.  Only rows of 200 KB and more would have 16 waves beyond (128256
+    // words of fp32, 1024 rows: 97 and 127).
     if (n_rows <= 512 && vocab * (int64_t)sizeof(T) >= 32768) GQ_LP(1024);
     else GQ_LP(256);
 #undef GQ_LP

@@ -585,9 +585,9 @@ def gemm_nt(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
 # ---- serving a quantised decoder --------------------------------------------------------------------------------
 
 class PagedCache(NamedTuple):
-    """Keys and values in pages of 16, 32, 64 or 128 tokens: e4m3 codes (``torch.float8_e4m3fn``) and one fp32 scale per
-    (page, kv head); value = code * scale.  Values lie by channel, (pages, heads, head_dim, tokens): the attention reads
-    them as an operand whose inner index is the token."""
+    """Keys and values, head_dim a multiple of 16 up to 128, in pages of 16, 32, 64 or 128 tokens: e4m3 codes
+    (``torch.float8_e4m3fn``) and one fp32 scale per (page, kv head); value = code * scale.  Values lie by channel, (pages,
+    heads, head_dim, tokens): the attention reads them as an operand whose inner index is the token."""
     k: torch.Tensor         # (pages, kv heads, page, head_dim)
     v: torch.Tensor         # (pages, kv heads, head_dim, page)
     k_scale: torch.Tensor   # (pages, kv heads)
@@ -643,8 +643,8 @@ def attention_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     """Attention over whole prompts: q (tokens, heads, head_dim), k / v (tokens, kv heads, head_dim) in fp16 or bf16, head_dim
     a multiple of 8 up to 128; strided views (slices of a merged q/k/v product) are taken as they are.  ``cu_seqlens``
     (sequences + 1) int32 says where the packed sequences begin and end (None: one sequence); rows behind the last are left
-    as they are.  Causal: token i of a sequence sees tokens 0..i.  ``scale`` defaults to head_dim ** -0.5.
-    ``out`` must not overlap q, k or v."""
+    as they are: undefined where no ``out`` is given.  Causal: token i of a sequence sees tokens 0..i.  ``scale`` defaults to
+    head_dim ** -0.5.  ``out`` must not overlap q, k or v."""
     return _serving.attention_prompt(q, k, v, cu_seqlens, causal, scale, out)
 
 
@@ -656,7 +656,8 @@ def kv_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, block_table: 
     ``cu_seqlens`` None: one new token for each sequence.  With ``cos`` / ``sin`` (positions, rotary_dim / 2) fp32 the keys are
     rotated on the way (rotary_dim even, 16 to head_dim), and q (tokens, heads, head_dim), if given, into ``q_out`` (which may
     be q), which is returned; pairs of channels are (j, j + rotary_dim / 2), or (2j, 2j + 1) if ``interleaved``.  See
-    gq_kv_append in gptq_amd.h for the scales and for tokens without a page or an angle."""
+    gq_kv_append in gptq_amd.h for the scales and for tokens without a page or an angle.  Query rows behind the last sequence are
+    left as they are: undefined where no ``q_out`` is given."""
     return _serving.kv_append(*cache, k, v, block_table, past_lens, cu_seqlens, q, cos, sin, interleaved, q_out)
 
 
@@ -667,7 +668,8 @@ def attention_paged(q: torch.Tensor, cache: PagedCache, block_table: torch.Tenso
     own position.  ``cu_seqlens`` None: one query token for each sequence (a decoder's step); several are a checked
     draft or a chunk of a prompt behind its cached beginning.  A row that sees nothing is 0; one that sees a token on no page
     is NaN (its sequence's others may be), and so is one that sees a token of a page whose scale is NaN.  The scratch memory
-    of long sequences comes from torch's allocator, a tensor per call.  ``out`` must not overlap q."""
+    of long sequences comes from torch's allocator, a tensor per call.  Rows behind the last sequence are left as they are:
+    undefined where no ``out`` is given.  ``out`` must not overlap q."""
     return _serving.attention_paged(q, *cache, block_table, seq_lens, cu_seqlens, scale, out)
 
 

@@ -429,8 +429,8 @@ typedef struct gq_paged_cache {
 
 /*
  * gq_attention_prompt: out = softmax(softmax_scale q k^T) v within each sequence; causal != 0: query i sees keys 0..i.
- * cu_seqlens NULL: one sequence of n_tokens (batch 1).  head_dim a multiple of 8 up to 128, sums and softmax in fp32, the
- * weights rounded to `dtype` for the second product. */
+ * cu_seqlens NULL: one sequence of n_tokens (batch 1).  head_dim a multiple of 8 up to 128, token strides of k and v from
+ * head_dim to 2^23; sums and softmax in fp32, the weights rounded to `dtype` for the second product. */
 typedef struct gq_attention_prompt_args {
     gq_rows out, q, k, v;
     int64_t dtype, n_tokens, n_heads, n_kv_heads, head_dim;
